@@ -1,5 +1,6 @@
 // module.cpp -- pybind11/torch binding of libgicc (opengda_b200._C).
 // Tensors are validated here; the kernels themselves live in libgicc.so.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -72,6 +73,124 @@ void gemm_tile_done_selftest(const at::Tensor& A, const at::Tensor& B, const at:
                                      static_cast<uint32_t*>(counters.data_ptr()), (uint32_t)skew_ns, cur_stream());
 }
 
+// ---- projections (ffn.cu, lora.cu) ----
+int fmt_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, " must be bfloat16 or float16");
+  return t.scalar_type() == at::kBFloat16 ? 1 : 0;
+}
+// A row-major matrix of `like`'s type and device with 16-byte aligned rows.
+void check_rows(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the inputs' device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the inputs' dtype");
+  TORCH_CHECK(t.dim() == 2, name, " must be 2-D");
+  TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX / 2, name, " is too large");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must be row-major (stride(1) == 1)");
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must have rows that do not overlap");
+}
+// The row pitch; a single row's stride says nothing, so it counts as dense.
+long long pitch_of(const at::Tensor& t) { return t.size(0) <= 1 ? std::max<int64_t>((t.size(1) + 7) / 8 * 8, 8) : t.stride(0); }
+
+at::Tensor out_or_empty(const c10::optional<at::Tensor>& out, int64_t rows, int64_t cols, const at::Tensor& like,
+                        std::initializer_list<at::Tensor> inputs) {
+  if (!out.has_value()) return at::empty({rows, cols}, like.options());
+  check_rows(*out, "out", like);
+  TORCH_CHECK(out->size(0) == rows && out->size(1) == cols, "out has the wrong shape");
+  for (const auto& t : inputs) at::assert_no_overlap(*out, t);
+  return *out;
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_linear(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
+                                                int64_t kind, bool save, c10::optional<at::Tensor> out, int64_t tile) {
+  const int fmt = fmt_of(x, "x");
+  check_rows(x, "x", x);
+  check_rows(w_gate, "w_gate", x);
+  check_rows(w_up, "w_up", x);
+  const int64_t T = x.size(0), H = x.size(1), I = w_gate.size(0);
+  TORCH_CHECK(w_gate.size(1) == H && w_up.size(1) == H && w_up.size(0) == I,
+              "x[T,H], w_gate[I,H], w_up[I,H] must share H and I");
+  const c10::cuda::CUDAGuard g(x.device());
+  at::Tensor h = out_or_empty(out, T, I, x, {x, w_gate, w_up});
+  at::Tensor saved;
+  if (save)
+    saved = at::empty({T > 0 ? (int64_t)gicc::ops::gated_saved_floats((int)T, (int)I) : 0}, x.options().dtype(at::kFloat));
+  if (T > 0)
+    gicc::ops::gated_linear(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), (int)T, (int)H, (int)I,
+                            pitch_of(x), pitch_of(w_gate), pitch_of(w_up), T == 1 ? std::max<int64_t>(I, h.stride(0)) : h.stride(0),
+                            (int)kind, fmt, save ? saved.data_ptr<float>() : nullptr, (int)tile, cur_stream());
+  return {h, saved};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::Tensor& dh, const at::Tensor& x,
+                                                                     const at::Tensor& w_gate, const at::Tensor& w_up,
+                                                                     const at::Tensor& saved, int64_t kind, bool need_dx,
+                                                                     bool need_dw) {
+  const int fmt = fmt_of(x, "x");
+  check_rows(x, "x", x);
+  check_rows(dh, "dh", x);
+  check_rows(w_gate, "w_gate", x);
+  check_rows(w_up, "w_up", x);
+  const int64_t T = x.size(0), H = x.size(1), I = w_gate.size(0);
+  TORCH_CHECK(w_gate.size(1) == H && w_up.size(1) == H && w_up.size(0) == I && dh.size(0) == T && dh.size(1) == I,
+              "dh[T,I], x[T,H], w_gate[I,H], w_up[I,H] must share T, H and I");
+  TORCH_CHECK(saved.is_cuda() && saved.device() == x.device() && saved.scalar_type() == at::kFloat && saved.is_contiguous() &&
+                  saved.numel() == (T > 0 ? (int64_t)gicc::ops::gated_saved_floats((int)T, (int)I) : 0),
+              "saved must be what gated_linear_forward kept for these shapes");
+  const c10::cuda::CUDAGuard g(x.device());
+  at::Tensor dx, dw;
+  if (need_dx) dx = at::empty({T, H}, x.options());
+  if (need_dw) dw = T > 0 ? at::empty({2, I, H}, x.options()) : at::zeros({2, I, H}, x.options());
+  if (T > 0 && (need_dx || need_dw)) {
+    at::Tensor work = at::empty({2 * T * gicc::ops::gated_grad_pitch((int)I)}, x.options());
+    uint8_t* pw = need_dw ? static_cast<uint8_t*>(dw.data_ptr()) : nullptr;
+    gicc::ops::gated_linear_backward(dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), saved.data_ptr<float>(),
+                                     work.data_ptr(), need_dx ? dx.data_ptr() : nullptr, pw, need_dw ? pw + 2 * I * H : nullptr,
+                                     (int)T, (int)H, (int)I, T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0),
+                                     pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, cur_stream());
+  }
+  return {dx, need_dw ? dw.select(0, 0) : at::Tensor(), need_dw ? dw.select(0, 1) : at::Tensor()};
+}
+
+at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& lora_a, const at::Tensor& lora_b,
+                       const at::Tensor& adapter, const c10::optional<at::Tensor>& scale, c10::optional<at::Tensor> out,
+                       int64_t tile) {
+  const int fmt = fmt_of(x, "x");
+  check_rows(x, "x", x);
+  check_rows(w, "w", x);
+  const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(w.size(1) == K, "x[T,K] and w[N,K] must share K");
+  for (const auto* t : {&lora_a, &lora_b})
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->dim() == 3 &&
+                    t->is_contiguous(),
+                "lora_a[L,r,K] and lora_b[L,N,r] must be contiguous, of x's dtype and on its device");
+  const int64_t L = lora_a.size(0), r = lora_a.size(1);
+  TORCH_CHECK(lora_a.size(2) == K && lora_b.size(0) == L && lora_b.size(1) == N && lora_b.size(2) == r,
+              "lora_a[L,r,K] and lora_b[L,N,r] must share L and r, and K and N with w[N,K]");
+  TORCH_CHECK(adapter.is_cuda() && adapter.device() == x.device() && adapter.scalar_type() == at::kInt && adapter.dim() == 1 &&
+                  adapter.size(0) == T && adapter.is_contiguous(),
+              "adapter must be a contiguous int32 tensor with one index per row of x, on its device");
+  const c10::cuda::CUDAGuard g(x.device());
+  at::Tensor s;
+  if (scale.has_value()) {
+    s = *scale;
+    TORCH_CHECK(s.is_cuda() && s.device() == x.device() && s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == L &&
+                    s.is_contiguous(),
+                "scale must be a contiguous float32 tensor with one factor per adapter, on x's device");
+  } else {
+    s = at::ones({L}, x.options().dtype(at::kFloat));
+  }
+  at::Tensor y = out_or_empty(out, T, N, x, {x, w, lora_a, lora_b, adapter, s});
+  TORCH_CHECK(L >= 1 && r >= 1, "at least one adapter of rank 8 or more");
+  if (T > 0) {
+    at::Tensor work = at::empty({(int64_t)gicc::ops::lora_work_bytes((int)T, (int)L, (int)r)}, x.options().dtype(at::kByte));
+    gicc::ops::lora_linear(x.data_ptr(), w.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr<int>(),
+                           s.data_ptr<float>(), y.data_ptr(), work.data_ptr(), (int)T, (int)K, (int)N, (int)L, (int)r,
+                           pitch_of(x), pitch_of(w), T == 1 ? std::max<int64_t>(N, y.stride(0)) : y.stride(0), fmt, (int)tile,
+                           cur_stream());
+  }
+  return y;
+}
+
 py::dict read_errors(bool clear) {
   gicc::ErrorRecord r = gicc::read_error_record(clear);
   py::dict d;
@@ -139,6 +258,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_fp32", &gemm_fp32, py::arg("A"), py::arg("B"), py::arg("out") = py::none(), py::arg("alpha") = 1.0,
         py::arg("bn") = 0,
         "fp32 C = alpha * A @ B^T on the tensor cores (three tf32 products)");
+  m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("act") = 0,
+        py::arg("save") = false, py::arg("out") = py::none(), py::arg("tile") = 0,
+        "h = act(x w_gate^T) * (x w_up^T); (h, what the backward pass needs)");
+  m.def("gated_linear_backward", &gated_linear_backward, py::arg("dh"), py::arg("x"), py::arg("w_gate"), py::arg("w_up"),
+        py::arg("saved"), py::arg("act") = 0, py::arg("need_dx") = true, py::arg("need_dw") = true,
+        "gradients of gated_linear: (dx, dw_gate, dw_up)");
+  m.def("lora_linear", &lora_linear, py::arg("x"), py::arg("w"), py::arg("lora_a"), py::arg("lora_b"), py::arg("adapter"),
+        py::arg("scale") = py::none(), py::arg("out") = py::none(), py::arg("tile") = 0,
+        "y = x w^T plus each row's low-rank adapter");
   m.def("gemm_tile_done_selftest", &gemm_tile_done_selftest, py::arg("A"), py::arg("B"), py::arg("counters"),
         py::arg("skew_ns") = 20000, "run the GEMM core with an epilogue that checks the tile-done ordering");
   m.def("config", [] {

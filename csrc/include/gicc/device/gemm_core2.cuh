@@ -106,6 +106,26 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(void* dst, const CUtensorM
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(m), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int x, int y,
+                                                 int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          ptx::smem_u32(dst)),
+      "l"(m), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// mma_pair that leaves the TMEM lanes whose bit of `skip` is set as they are (words 0..3: the
+// leader's 128 rows, 4..7: the peer's).
+__device__ __forceinline__ void mma_pair_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate, const uint32_t* skip) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(skip[0]), "r"(skip[1]), "r"(skip[2]), "r"(skip[3]),
+      "r"(skip[4]), "r"(skip[5]), "r"(skip[6]), "r"(skip[7])
+      : "memory");
+}
 __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          uint32_t accumulate) {
   asm volatile(
@@ -185,6 +205,24 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint4 v) {
                : "memory");
 }
 __device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
+// Schedules with `static constexpr bool kOwnOperands = true` place their operands themselves
+// (other majors, 16-bit types, tensor maps or k-blocks than the plain GEMM's):
+//   issue_loads_pair(ti, kb, crank, sA, sB, bar)  this CTA's loads of one k-block, kStageBytes in all
+//   idesc(ti), a_desc(ti, addr, k), b_desc(ti, addr, k)  the MMA descriptors of k-step k of a stage
+//   lane_skip(ti, kb, skip)  true: this k-block leaves the TMEM lanes set in skip[8] alone
+template <class S, class = void>
+struct sched_own : std::false_type {};
+template <class S>
+struct sched_own<S, std::void_t<decltype(S::kOwnOperands)>> : std::integral_constant<bool, S::kOwnOperands> {};
+
+// Epilogues with `static constexpr bool kGated = true` (NH = 2) get columns c of both halves at
+// once: gate(ti, row, c, lo, hi) combines 32 columns of half 0 and half 1 into hi, which is then
+// stored like one half's columns.
+template <class E, class = void>
+struct epi_gated : std::false_type {};
+template <class E>
+struct epi_gated<E, std::void_t<decltype(E::kGated)>> : std::integral_constant<bool, E::kGated> {};
 
 // Options of the operand loads (the plain GEMM's tuning; the fused kernels use none):
 // l2hint 1 = A kept in L2 / B streamed, 2 = the reverse; prefetch = k-steps ahead at which
@@ -352,7 +390,9 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
           const uint32_t bar = map_to(ptx::smem_u32(&full[stage]), 0);
           if (leader) ptx::mbar_arrive_expect_tx(&full[stage], 2 * Cf::kStageBytes);
           const int a_y = ti.a_row + (int)crank * BM;
-          if (lopt.l2hint == 0) {
+          if constexpr (sched_own<Sched>::value) {
+            sched.issue_loads_pair(ti, kb, (int)crank, sA + stage * kABytes, sB + stage * NH * kBBytes, bar);
+          } else if (lopt.l2hint == 0) {
             tma_load_2d_pair(sA + stage * kABytes, tmA, bar, kb * kKE, a_y);
 #pragma unroll
             for (int h = 0; h < NH; ++h)
@@ -365,7 +405,7 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
               tma_load_2d_pair_hint(sB + (stage * NH + h) * kBBytes, tmB, bar, kb * kKE,
                                     ti.b_row + h * BN2 + (int)crank * (BN2 / 2), pol_b);
           }
-          if (lopt.prefetch > 0 && kb + lopt.prefetch < ti.kb1) {
+          if (!sched_own<Sched>::value && lopt.prefetch > 0 && kb + lopt.prefetch < ti.kb1) {
             const int px = (kb + lopt.prefetch) * kKE;
             tma_prefetch_2d(tmA, px, a_y);
 #pragma unroll
@@ -391,7 +431,7 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
   } else if (warp == 1) {
     if (lane == 0 && leader) {
       // ---------------- MMA issuer (leader CTA) ----------------
-      constexpr uint32_t idesc = kTf32 ? ptx::idesc_tf32_f32(2 * BM, BN2) : ptx::idesc_bf16_f32(2 * BM, BN2);
+      constexpr uint32_t idesc0 = kTf32 ? ptx::idesc_tf32_f32(2 * BM, BN2) : ptx::idesc_bf16_f32(2 * BM, BN2);
       const uint32_t peer = 1;
       int stage = 0;
       uint32_t phase = 0;
@@ -423,14 +463,26 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
         auto issue = [&](int st, int kb, int h0, int h1) {
           const uint32_t a0 = ptx::smem_u32(sA + st * kABytes);
           const uint32_t b0 = ptx::smem_u32(sB + st * NH * kBBytes);
+          uint32_t idesc = idesc0;
+          uint32_t skip[8];
+          bool lanes = false;
+          if constexpr (sched_own<Sched>::value) {
+            idesc = sched.idesc(ti);
+            lanes = sched.lane_skip(ti, kb, skip);
+          }
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t ad = ptx::sdesc_kmajor_sw128(a0 + k * 32);
+            uint64_t ad;
+            if constexpr (sched_own<Sched>::value) ad = sched.a_desc(ti, a0, k);
+            else ad = ptx::sdesc_kmajor_sw128(a0 + k * 32);
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
               if (h < h0 || h >= h1) continue;
-              const uint64_t bd = ptx::sdesc_kmajor_sw128(b0 + h * kBBytes + k * 32);
-              if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc, (kb > ti.kb0 || k > 0) ? 1u : 0u);
+              uint64_t bd;
+              if constexpr (sched_own<Sched>::value) bd = sched.b_desc(ti, b0 + h * kBBytes, k);
+              else bd = ptx::sdesc_kmajor_sw128(b0 + h * kBBytes + k * 32);
+              if (sched_own<Sched>::value && lanes) mma_pair_lanes(d + h * BN2, ad, bd, idesc, 1u, skip);
+              else if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc, (kb > ti.kb0 || k > 0) ? 1u : 0u);
               else mma_pair(d + h * BN2, ad, bd, idesc, (kb > ti.kb0 || k > 0) ? 1u : 0u);
             }
           }
@@ -562,61 +614,93 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
       ptx::tc_fence_after();
       const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * NH * BN2;
       epi.begin_tile(ti, row);
-#pragma unroll 1
-      for (int h = 0; h < NH; ++h) {
-        // the barrier that frees what this warp has read: the accumulator (NH = 1) or half h
-        const uint32_t free_bar = (NH == 1 ? acc : h) ? tempty_leader1 : tempty_leader0;
-#pragma unroll 1
-        for (int c = 0; c < kSeg; c += kW) {
-          // kW columns: every TMEM load issued before one wait (each wait is a round trip)
-          const int col0 = h * BN2 + part * kSeg + c;
-          uint32_t r[kW];
+      // 32 columns from `col` of this thread's row: through a shared-memory box and TMA, or
+      // from the registers
+      auto put = [&](const uint32_t* ri, int col) {
+        if constexpr (kStaged) {
+          if (epi.staged()) {
+            uint8_t* box = my_boxes + (box_turn & 1) * Cf::kBoxBytes;
+            ++box_turn;
+            if (lane == 0) bulk_wait_read_1();  // the store issued from this box two chunks ago
+            __syncwarp();
+            uint4 v[4];
+            epi.pack(ri, v);
+            // row `lane` of the box (64 bytes); the 16-byte pieces are written in an
+            // order rotated by lane/2, so each group of 8 lanes covers all 32 banks
+            const uint32_t rowaddr = ptx::smem_u32(box) + lane * 64;
 #pragma unroll
-          for (int i = 0; i < kW / 32; ++i) ptx::tmem_ld32(tbase + col0 + 32 * i, r + 32 * i);
-          ptx::tmem_ld_wait();
-          // Epilogues that publish finished tiles free the last half only after tile_done
-          // (below); half 0 of a 512-column accumulator can go back at once, because the
-          // next tile's epilogue cannot start before half 1 is free.
-          if (!Epi::kNeedsTileDone || h + 1 < NH) {
-            if (c + kW >= kSeg) {
-              ptx::tc_fence_before();
-              __syncwarp();
-              if (lane == 0) arrive_cluster(free_bar);
+            for (int j = 0; j < 4; ++j) {
+              const int cj = (j + (int)(lane >> 1)) & 3;
+              const uint4 w = cj == 0 ? v[0] : cj == 1 ? v[1] : cj == 2 ? v[2] : v[3];
+              st_shared_v4(rowaddr + cj * 16, w);
             }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (epi.chunk_in_bounds(ti, q * 32, col))
+                ptx::tma_store_2d(epi.tmap(), box, ti.n0 + col, ti.m0 + q * 32);
+              ptx::bulk_commit();  // a group per box, empty when out of bounds, so the wait counts boxes
+            }
+            return;
           }
+        }
+        epi.store(ti, row, col, ri);
+      };
+      if constexpr (epi_gated<Epi>::value) {
+        // This warp's first 32 columns of both halves, then the other 96 of half 0 into registers
+        // (all 128 at once would spill), which frees half 0 for the next tile's first k-steps
+        // after a quarter of the drain; half 1 follows 32 columns at a time.
+        static_assert(!epi_gated<Epi>::value || (NH == 2 && !Epi::kNeedsTileDone), "gated epilogue: 256 x 512 tiles");
+        uint32_t lo[kSeg - 32], hi[32];
+        const int c0 = part * kSeg;
+        ptx::tmem_ld32(tbase + c0, lo);
+        ptx::tmem_ld32(tbase + BN2 + c0, hi);
+        ptx::tmem_ld_wait();
+        epi.gate(ti, row, c0, lo, hi);
+        put(hi, c0);
 #pragma unroll
-          for (int i = 0; i < kW / 32; ++i) {
-            const int col = col0 + 32 * i;
-            const uint32_t* ri = r + 32 * i;
-            bool done = false;
-            if constexpr (kStaged) {
-              if (epi.staged()) {
-                uint8_t* box = my_boxes + (box_turn & 1) * Cf::kBoxBytes;
-                ++box_turn;
-                if (lane == 0) bulk_wait_read_1();  // the store issued from this box two chunks ago
-                __syncwarp();
-                uint4 v[4];
-                epi.pack(ri, v);
-                // row `lane` of the box (64 bytes); the 16-byte pieces are written in an
-                // order rotated by lane/2, so each group of 8 lanes covers all 32 banks
-                const uint32_t rowaddr = ptx::smem_u32(box) + lane * 64;
+        for (int i = 1; i < kSeg / 32; ++i) ptx::tmem_ld32(tbase + c0 + 32 * i, lo + 32 * (i - 1));
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(tempty_leader0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int cj = (j + (int)(lane >> 1)) & 3;
-                  const uint4 w = cj == 0 ? v[0] : cj == 1 ? v[1] : cj == 2 ? v[2] : v[3];
-                  st_shared_v4(rowaddr + cj * 16, w);
-                }
-                ptx::fence_proxy_async_smem();
+        for (int i = 1; i < kSeg / 32; ++i) {
+          ptx::tmem_ld32(tbase + BN2 + c0 + 32 * i, hi);
+          ptx::tmem_ld_wait();
+          if (i + 1 == kSeg / 32) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(tempty_leader1);
+          }
+          epi.gate(ti, row, c0 + 32 * i, lo + 32 * (i - 1), hi);
+          put(hi, c0 + 32 * i);
+        }
+      } else {
+#pragma unroll 1
+        for (int h = 0; h < NH; ++h) {
+          // the barrier that frees what this warp has read: the accumulator (NH = 1) or half h
+          const uint32_t free_bar = (NH == 1 ? acc : h) ? tempty_leader1 : tempty_leader0;
+#pragma unroll 1
+          for (int c = 0; c < kSeg; c += kW) {
+            // kW columns: every TMEM load issued before one wait (each wait is a round trip)
+            const int col0 = h * BN2 + part * kSeg + c;
+            uint32_t r[kW];
+#pragma unroll
+            for (int i = 0; i < kW / 32; ++i) ptx::tmem_ld32(tbase + col0 + 32 * i, r + 32 * i);
+            ptx::tmem_ld_wait();
+            // Epilogues that publish finished tiles free the last half only after tile_done
+            // (below); half 0 of a 512-column accumulator can go back at once, because the
+            // next tile's epilogue cannot start before half 1 is free.
+            if (!Epi::kNeedsTileDone || h + 1 < NH) {
+              if (c + kW >= kSeg) {
+                ptx::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                  if (epi.chunk_in_bounds(ti, q * 32, col))
-                    ptx::tma_store_2d(epi.tmap(), box, ti.n0 + col, ti.m0 + q * 32);
-                  ptx::bulk_commit();  // a group per box, empty when out of bounds, so the wait counts boxes
-                }
-                done = true;
+                if (lane == 0) arrive_cluster(free_bar);
               }
             }
-            if (!done) epi.store(ti, row, col, ri);
+#pragma unroll
+            for (int i = 0; i < kW / 32; ++i) put(r + 32 * i, col0 + 32 * i);
           }
         }
       }

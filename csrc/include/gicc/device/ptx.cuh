@@ -309,6 +309,16 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same, leaving the TMEM lanes (rows of A) whose bit of `skip` is set as they are.
+__device__ __forceinline__ void mma_f16_ss_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate, const uint32_t* skip) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(skip[0]), "r"(skip[1]), "r"(skip[2]), "r"(skip[3])
+      : "memory");
+}
 // D[tmem] (+)= A[smem] * B[smem]^T, tf32 inputs (fp32 words; the MMA uses their tf32 part),
 // f32 accumulate; K = 8 per instruction (32 bytes of a 128-byte swizzle row, as kind::f16).
 __device__ __forceinline__ void mma_tf32_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -362,11 +372,26 @@ __host__ __device__ constexpr uint32_t idesc_tf32_f32(int M, int N) {
   return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// kind::f16 with either 16-bit type (fmt 0 = f16, 1 = bf16, the same for A and B) and either
+// operand K-major (0) or MN-major (1).
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, int fmt, int a_mn, int b_mn) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
 // Shared-memory matrix descriptor, K-major operand, 128-byte swizzle:
 // rows of 128 B (64 bf16), 8-row swizzle atoms 1024 B apart (SBO), LBO unused (1),
 // descriptor version 1 at bits [46,48), layout 2 (SWIZZLE_128B) at bits [61,64).
 __device__ __forceinline__ uint64_t sdesc_kmajor_sw128(uint32_t smem_addr) {
   return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Shared-memory matrix descriptor, MN-major operand, 128-byte swizzle: rows of 128 B hold 64
+// consecutive M (or N) elements of one k; 8 k make a 1024-byte swizzle atom (SBO: the next 8 k),
+// and the next 64 M (or N) elements follow `mn_step` bytes later (LBO).
+__device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t smem_addr, uint32_t mn_step) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)(mn_step >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
@@ -382,8 +407,34 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// fmt 0 = f16, 1 = bf16 (the kind::f16 operand codes)
+__device__ __forceinline__ uint32_t pack_16x2(float lo, float hi, int fmt) {
+  return fmt ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+__device__ __forceinline__ float f16_to_f32(uint16_t v) {
+  float f;
+  asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(v));
+  return f;
+}
+__device__ __forceinline__ float from_16(uint16_t v, int fmt) {
+  return fmt ? __uint_as_float((uint32_t)v << 16) : f16_to_f32(v);
+}
+
+// ---------------------------------------------------------------------------------------
+// Programmatic dependent launch: `griddep_launch` lets the next kernel of the stream (one
+// launched with the programmatic attribute) start once every CTA has called it or ended;
+// `griddep_wait` waits until the previous kernel has ended and its stores are visible.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 }  // namespace ptx
 }  // namespace gicc

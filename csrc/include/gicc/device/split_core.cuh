@@ -1,0 +1,283 @@
+// split_core.cuh -- tcgen05 projection core for few rows: one output tile per thread-block
+// cluster, the depth K split over the cluster's CTAs.
+//
+//   D_i[rows, cols] = X[rows, K] * W_i[cols, K]^T,  i = 0 .. kAccs-1, f32 accumulate
+//
+// With few rows the product is a stream of the weights from HBM, and the output has too few
+// tiles to give every SM one.  So a cluster of S CTAs takes one tile of up to 128 rows x bn
+// columns, each CTA runs its share of the k-blocks through its own TMA ring and accumulators
+// (rows in TMEM lanes, columns of weight i at i * bn), writes its f32 partial to its own
+// shared memory, and after a cluster barrier every CTA sums a slice of the tile over all S
+// partials (distributed shared memory, in rank order, so results do not depend on timing)
+// and hands it to the Op's emit().  One launch, no workspace, no atomics.
+//
+// Warp roles: 0 producer, 1 TMEM + MMA, 2..5 TMEM readers; all six sum and store.  Every wait
+// is bounded; all CTAs of a cluster always reach both cluster barriers.
+#pragma once
+#include <cstdint>
+
+#include "gicc/device/gemm_core2.cuh"
+
+namespace gicc {
+namespace gemm {
+namespace split {
+
+constexpr int kRows = 128;              // rows of a tile (TMEM lanes)
+constexpr int kThreads = 192;
+constexpr int kMaxSplit = 8;            // portable cluster size
+constexpr int kMaxCols = 128;           // columns of one weight per tile
+constexpr int kMaxStages = 12;
+constexpr uint32_t kXBytes = kRows * BK * 2;
+constexpr uint32_t kBarBytes = (2 * kMaxStages + 2) * 8 + 16;
+
+struct Shape {
+  int T, N, K;   // rows of X, rows of each W, depth
+  int bn;        // columns per tile and weight: a multiple of 16
+  int xrows;     // rows of an X box: min(128, T rounded up to 8)
+  int stages;
+};
+
+__host__ __device__ constexpr uint32_t stage_bytes(int accs, int bn) { return kXBytes + accs * bn * BK * 2; }
+// floats between two rows of a partial: + 4 keeps the 16-byte writes of 8 lanes on 32 banks
+__host__ __device__ constexpr int pitch(int accs, int bn) { return accs * bn + 4; }
+__host__ __device__ constexpr uint32_t ring_bytes(int accs, int bn, int stages, int rows) {
+  const uint32_t ring = stages * stage_bytes(accs, bn), part = rows * pitch(accs, bn) * 4;
+  return ((ring > part ? ring : part) + 127) / 128 * 128;
+}
+__host__ __device__ constexpr uint32_t tmem_cols(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256; }
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four columns of an output row in its 16-bit type: one 8-byte store where C's base and pitch
+// allow it (vec) and all four columns exist, else element stores.
+__device__ __forceinline__ void store4_16(uint16_t* row, int col, int N, const float* v, int fmt, int vec) {
+  const uint32_t a = ptx::pack_16x2(v[0], v[1], fmt), b = ptx::pack_16x2(v[2], v[3], fmt);
+  if (vec && col + 4 <= N) {
+    *reinterpret_cast<uint2*>(row + col) = make_uint2(a, b);
+  } else {
+    if (col < N) row[col] = (uint16_t)a;
+    if (col + 1 < N) row[col + 1] = (uint16_t)(a >> 16);
+    if (col + 2 < N) row[col + 2] = (uint16_t)b;
+    if (col + 3 < N) row[col + 3] = (uint16_t)(b >> 16);
+  }
+}
+
+// Op: kAccs (weights multiplied side by side), fmt() (16-bit type), and
+//   prepare(smem_extra, t0, ...)   by all threads before the pipeline starts
+//   extra_blocks(c, S, e0, e1)     this CTA's further k-blocks after the weights'
+//   extra_wait()                   by the producer before the first of them
+//   extra_loads(e, sh, t0, n0, sX, sW, bar)   loads of one (stage_tx() bytes, as a weight block)
+//   extra_mma(e, d, xs, ws, idesc)            its MMAs
+//   emit(row, col, v)              v[i][4]: four columns of weight i of one valid row
+//   finish()                       by all threads, last
+template <class Op>
+__device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtensorMap* tmW0, const CUtensorMap* tmW1,
+                                           const Shape& sh, Op& op, ErrorRecord* err, uint64_t timeout_ns) {
+  constexpr int A = Op::kAccs;
+  extern __shared__ uint8_t split_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(split_smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stages = sh.stages;
+  const uint32_t wbytes = sh.bn * BK * 2;
+  uint8_t* sX = smem;
+  uint8_t* sW = smem + stages * kXBytes;  // per stage: A consecutive blocks of wbytes
+  uint8_t* after = smem + ring_bytes(A, sh.bn, stages, kRows);
+  uint64_t* full = reinterpret_cast<uint64_t*>(after);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint64_t* drain = tfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* part = reinterpret_cast<float*>(smem);  // after the last MMA: this CTA's partial
+
+  const uint32_t warp = ptx::warp_id();
+  const uint32_t lane = ptx::lane_id();
+  const int S = (int)cluster_size();
+  const int c = (int)pair::cta_rank();
+  const int n0 = (int)(blockIdx.x / S) * sh.bn;
+  const int t0 = (int)blockIdx.y * kRows;
+  const int rows = min(kRows, sh.T - t0);
+  const uint32_t ncols = tmem_cols(A * sh.bn);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    ptx::mbar_init(tfull, 1);
+    ptx::mbar_init(drain, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(tmX);
+    ptx::prefetch_tmap(tmW0);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, ncols);
+    ptx::tmem_relinquish();
+  }
+  op.prepare(after + kBarBytes, t0, err);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int nkb = (sh.K + BK - 1) / BK;
+  const int kb0 = (int)((long long)nkb * c / S), kb1 = (int)((long long)nkb * (c + 1) / S);
+  int e0, e1;
+  op.extra_blocks(c, S, e0, e1);
+  const int steps = (kb1 - kb0) + (e1 - e0);  // >= 1: the host takes S <= nkb
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t tx = sh.xrows * BK * 2 + A * wbytes;
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      for (int i = 0; i < steps; ++i) {
+        if (i == kb1 - kb0) op.extra_wait();
+        if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
+          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
+          *abort_flag = 1;
+          break;
+        }
+        ptx::mbar_arrive_expect_tx(&full[stage], tx);
+        uint8_t* x = sX + stage * kXBytes;
+        uint8_t* w = sW + stage * A * wbytes;
+        if (i < kb1 - kb0) {
+          const int kx = (kb0 + i) * BK;
+          ptx::tma_load_2d(x, tmX, &full[stage], kx, t0);
+          ptx::tma_load_2d(w, tmW0, &full[stage], kx, n0);
+          if constexpr (A == 2) ptx::tma_load_2d(w + wbytes, tmW1, &full[stage], kx, n0);
+        } else {
+          op.extra_loads(e0 + i - (kb1 - kb0), t0, n0, x, w, &full[stage]);
+        }
+        issued = i + 1;
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (*abort_flag) {
+        // Let the TMA loads already issued land before the CTA's smem is used again.
+        for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+          ptx::mbar_wait(&full[i % stages], (i / stages) & 1, 20000000ull, nullptr);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::idesc_f16_f32(kRows, sh.bn, op.fmt(), 0, 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      int i = 0;
+      for (; i < steps; ++i) {
+        if (!ptx::mbar_wait(&full[stage], phase, timeout_ns, abort_flag)) {
+          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 2, 0);
+          *abort_flag = 1;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t x = ptx::smem_u32(sX + stage * kXBytes);
+        const uint32_t w = ptx::smem_u32(sW + stage * A * wbytes);
+        if (i < kb1 - kb0) {
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t ad = ptx::sdesc_kmajor_sw128(x + k * 32);
+#pragma unroll
+            for (int a = 0; a < A; ++a)
+              ptx::mma_f16_ss(tmem + a * sh.bn, ad, ptx::sdesc_kmajor_sw128(w + a * wbytes + k * 32), idesc,
+                              (i > 0 || k > 0) ? 1u : 0u);
+          }
+        } else {
+          op.extra_mma(e0 + i - (kb1 - kb0), tmem, x, w, idesc);
+        }
+        ptx::mma_commit(&empty[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (i == steps) {
+        ptx::mma_commit(tfull);
+      } else if (i > 0) {  // aborted: wait for the MMAs in flight before TMEM is released
+        ptx::mma_commit(drain);
+        ptx::mbar_wait(drain, 0, 20000000ull, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const int row = q * 32 + (int)lane;
+    if (!ptx::mbar_wait_long(tfull, 0, timeout_ns, abort_flag)) {
+      if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 3, 0);
+      *abort_flag = 1;
+    } else if (q * 32 < rows) {
+      ptx::tc_fence_after();
+      const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16);
+      float* dst = part + row * pitch(A, sh.bn);
+      for (int col = 0; col < A * sh.bn; col += 16) {
+        uint32_t r[16];
+        ptx::tmem_ld16(tbase + col, r);
+        ptx::tmem_ld_wait();
+        if (row < rows) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(dst + col + 4 * j) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  pair::cluster_sync();  // every CTA's partial is in place
+  if (!*abort_flag) {
+    const int g4 = sh.bn / 4;  // groups of four columns per row
+    const int groups = rows * g4;
+    const int j1 = (int)((long long)groups * (c + 1) / S);
+    const uint32_t base = ptx::smem_u32(part);
+    for (int j = (int)((long long)groups * c / S) + (int)threadIdx.x; j < j1; j += kThreads) {
+      const int row = j / g4, col = (j - row * g4) * 4;
+      float v[A][4];
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+        const uint32_t off = base + (row * pitch(A, sh.bn) + a * sh.bn + col) * 4;
+        float4 p[kMaxSplit];
+#pragma unroll
+        for (int s = 0; s < kMaxSplit; ++s)
+          if (s < S) p[s] = ld_cluster_f4(pair::map_to(off, s));
+        v[a][0] = p[0].x;
+        v[a][1] = p[0].y;
+        v[a][2] = p[0].z;
+        v[a][3] = p[0].w;
+#pragma unroll
+        for (int s = 1; s < kMaxSplit; ++s)
+          if (s < S) {
+            v[a][0] += p[s].x;
+            v[a][1] += p[s].y;
+            v[a][2] += p[s].z;
+            v[a][3] += p[s].w;
+          }
+      }
+      op.emit(t0 + row, n0 + col, v);
+    }
+  }
+  op.finish();
+  pair::cluster_sync();  // no CTA leaves while its partial is being read
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, ncols);
+  }
+}
+
+}  // namespace split
+}  // namespace gemm
+}  // namespace gicc

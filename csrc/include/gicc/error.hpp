@@ -41,6 +41,7 @@ enum Where : int {
   W_BOUNDS = 11,
   W_PINGPONG = 12,
   W_RING_MM = 13,
+  W_ADAPTER = 14,
 };
 
 struct ErrorRecord {

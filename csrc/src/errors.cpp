@@ -92,6 +92,7 @@ const char* where_name(int w) {
     case W_BOUNDS: return "bounds";
     case W_PINGPONG: return "pingpong";
     case W_RING_MM: return "ring matmul";
+    case W_ADAPTER: return "adapter index";
   }
   return "?";
 }
