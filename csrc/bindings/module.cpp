@@ -3,6 +3,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "gicc/config.hpp"
@@ -124,7 +125,7 @@ std::tuple<at::Tensor, at::Tensor> gated_linear(const at::Tensor& x, const at::T
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::Tensor& dh, const at::Tensor& x,
                                                                      const at::Tensor& w_gate, const at::Tensor& w_up,
                                                                      const at::Tensor& saved, int64_t kind, bool need_dx,
-                                                                     bool need_dw) {
+                                                                     bool need_dw, int64_t tile) {
   const int fmt = fmt_of(x, "x");
   check_rows(x, "x", x);
   check_rows(dh, "dh", x);
@@ -141,14 +142,56 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::T
   if (need_dx) dx = at::empty({T, H}, x.options());
   if (need_dw) dw = T > 0 ? at::empty({2, I, H}, x.options()) : at::zeros({2, I, H}, x.options());
   if (T > 0 && (need_dx || need_dw)) {
-    at::Tensor work = at::empty({2 * T * gicc::ops::gated_grad_pitch((int)I)}, x.options());
+    at::Tensor work = at::empty({(int64_t)gicc::ops::gated_grad_bytes((int)T, (int)I)},
+                                 x.options().dtype(at::kByte));
     uint8_t* pw = need_dw ? static_cast<uint8_t*>(dw.data_ptr()) : nullptr;
     gicc::ops::gated_linear_backward(dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), saved.data_ptr<float>(),
                                      work.data_ptr(), need_dx ? dx.data_ptr() : nullptr, pw, need_dw ? pw + 2 * I * H : nullptr,
                                      (int)T, (int)H, (int)I, T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0),
-                                     pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, cur_stream());
+                                     pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, (int)tile, cur_stream());
   }
   return {dx, need_dw ? dw.select(0, 0) : at::Tensor(), need_dw ? dw.select(0, 1) : at::Tensor()};
+}
+
+// The autograd node (C++, so that neither pass takes the interpreter's lock for its own work).
+struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w_gate,
+                            const at::Tensor& w_up, int64_t kind) {
+    auto hs = gated_linear(x, w_gate, w_up, kind, true, c10::nullopt, 0);
+    ctx->save_for_backward({x, w_gate, w_up, std::get<1>(hs)});
+    ctx->saved_data["kind"] = kind;
+    return std::get<0>(hs);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
+    torch::autograd::variable_list out(4);
+    if (!grads[0].defined()) return out;
+    std::tuple<at::Tensor, at::Tensor, at::Tensor> d;
+    {
+      const at::AutoGradMode off(false);
+      d = gated_linear_backward(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3], ctx->saved_data["kind"].toInt(),
+                                need_x, need_g || need_u, 0);
+    }
+    if (need_x) out[0] = std::get<0>(d);
+    if (need_g) out[1] = std::get<1>(d);
+    if (need_u) out[2] = std::get<2>(d);
+    if (at::GradMode::is_enabled()) {  // create_graph: there is no second derivative to go through
+      torch::autograd::variable_list defined;
+      for (const auto& t : out)
+        if (t.defined()) defined.push_back(t);
+      torch::autograd::DelayedError error("gated_linear: the backward pass is not differentiable", defined.size());
+      defined = error.apply(std::move(defined));
+      size_t k = 0;
+      for (auto& t : out)
+        if (t.defined()) t = defined[k++];
+    }
+    return out;
+  }
+};
+
+at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, int64_t kind) {
+  return GatedLinearFn::apply(x, w_gate, w_up, kind);
 }
 
 at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& lora_a, const at::Tensor& lora_b,
@@ -261,8 +304,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("act") = 0,
         py::arg("save") = false, py::arg("out") = py::none(), py::arg("tile") = 0,
         "h = act(x w_gate^T) * (x w_up^T); (h, what the backward pass needs)");
+  m.def("gated_linear_autograd", &gated_linear_autograd, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("act") = 0,
+        "gated_linear as a node of the autograd graph");
   m.def("gated_linear_backward", &gated_linear_backward, py::arg("dh"), py::arg("x"), py::arg("w_gate"), py::arg("w_up"),
-        py::arg("saved"), py::arg("act") = 0, py::arg("need_dx") = true, py::arg("need_dw") = true,
+        py::arg("saved"), py::arg("act") = 0, py::arg("need_dx") = true, py::arg("need_dw") = true, py::arg("tile") = 0,
         "gradients of gated_linear: (dx, dw_gate, dw_up)");
   m.def("lora_linear", &lora_linear, py::arg("x"), py::arg("w"), py::arg("lora_a"), py::arg("lora_b"), py::arg("adapter"),
         py::arg("scale") = py::none(), py::arg("out") = py::none(), py::arg("tile") = 0,

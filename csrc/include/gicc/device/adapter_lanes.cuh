@@ -14,25 +14,37 @@ namespace lora {
 constexpr int kMaxAdapters = 8192;
 constexpr int kWords = kMaxAdapters / 32;
 
-template <int ROWS>
+// MASKS false: only the list and the rows' slots.
+template <int ROWS, bool MASKS = true>
 struct LaneLists {
+  uint32_t skip[MASKS ? ROWS : 1][ROWS / 32];  // per distinct adapter: lanes that are not its
   uint32_t used[kWords];            // bit a: some row uses adapter a
   int before[kWords];               // distinct adapters below word w's
-  uint32_t skip[ROWS][ROWS / 32];   // per distinct adapter: lanes that are not its
   int list[ROWS];                   // distinct adapters, ascending
   int n;
 
-  // All threads of the block; synchronises.  An index outside [-1, L) is reported and its row
-  // treated as having no adapter.
+  // All threads of the block (at least ROWS / 2); synchronises.  An index outside [-1, L) is
+  // reported and its row treated as having no adapter.
   __device__ void build(const int* adapter, int t0, int T, int L, ErrorRecord* err) {
     const int words = (L + 31) / 32;
-    for (int w = threadIdx.x; w < words; w += blockDim.x) used[w] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < ROWS; i += blockDim.x) {
-      const int a = at(adapter, t0 + i, T, L);
-      if (a >= 0) atomicOr(&used[a >> 5], 1u << (a & 31));
-      else if (a < -1) report_error(err, GICC_ERANGE, W_ADAPTER, -1, -1, (unsigned)adapter[t0 + i], (unsigned)L);
+    int mine[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = threadIdx.x + k * blockDim.x, t = t0 + i;
+      mine[k] = -1;
+      if (i < ROWS && t < T) {
+        const int a = adapter[t];
+        if (a >= 0 && a < L) mine[k] = a;
+        else if (a != -1) report_error(err, GICC_ERANGE, W_ADAPTER, -1, -1, (unsigned)a, (unsigned)L);
+      }
     }
+    for (int w = threadIdx.x; w < words; w += blockDim.x) used[w] = 0;
+    if (MASKS)
+      for (int i = threadIdx.x; i < ROWS * (ROWS / 32); i += blockDim.x) skip[0][i] = ~0u;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (mine[k] >= 0) atomicOr(&used[mine[k] >> 5], 1u << (mine[k] & 31));
     __syncthreads();
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
@@ -54,23 +66,17 @@ struct LaneLists {
       if (lane == 0) n = run;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n * (ROWS / 32); i += blockDim.x) skip[0][i] = ~0u;
-    __syncthreads();
-    for (int i = threadIdx.x; i < ROWS; i += blockDim.x) {
-      const int s = slot(at(adapter, t0 + i, T, L));
-      if (s >= 0) atomicAnd(&skip[s][i >> 5], ~(1u << (i & 31)));
+    if (MASKS) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (mine[k] >= 0) atomicAnd(&skip[slot(mine[k])][i >> 5], ~(1u << (i & 31)));
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
-  // the row's adapter, -1 for none, -2 for an index outside [-1, L)
-  __device__ static int at(const int* adapter, int t, int T, int L) {
-    if (t >= T) return -1;
-    const int a = adapter[t];
-    return a >= -1 && a < L ? a : -2;
-  }
-  __device__ int slot(int a) const {
-    return a < 0 ? -1 : before[a >> 5] + __popc(used[a >> 5] & ((1u << (a & 31)) - 1u));
-  }
+  // a's place in the list, for an adapter that some row uses
+  __device__ int slot(int a) const { return before[a >> 5] + __popc(used[a >> 5] & ((1u << (a & 31)) - 1u)); }
 };
 
 }  // namespace lora

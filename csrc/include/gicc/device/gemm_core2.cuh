@@ -66,7 +66,10 @@ struct PairCfg {
   // boxes per epilogue warp after the barrier area.
   static constexpr uint32_t kBoxBytes = 32 * 32 * 2;
   static constexpr uint32_t kSmemBytesStaged = kSmemBytes + kEpiWarps * 2 * kBoxBytes;
-  static_assert(kSmemBytesStaged <= 227 * 1024, "shared memory");
+  // Epilogues with swizzled boxes: as many boxes per warp as fit, on 512-byte boundaries.
+  static constexpr int kSwzBoxes = NH == 1 ? 4 : 2;
+  static constexpr uint32_t kSmemBytesSwizzled = kSmemBytes + 256 + kEpiWarps * kSwzBoxes * kBoxBytes;
+  static_assert(kSmemBytesSwizzled <= 227 * 1024, "shared memory");
 };
 // The 256 x 256 configuration's constants, kept under their original names.
 constexpr int kStages = PairCfg<1>::kStages;
@@ -200,25 +203,65 @@ struct epi_staged : std::false_type {};
 template <class E>
 struct epi_staged<E, std::void_t<decltype(E::kStagedStore)>> : std::integral_constant<bool, E::kStagedStore> {};
 
+// Staged epilogues with `static constexpr bool kRowStores = true` store a C that TMA cannot take
+// from the same box, row by row (Epi::store_rows(ti, row0, col, box, lane), by the whole warp).
+template <class E, class = void>
+struct epi_rows : std::false_type {};
+template <class E>
+struct epi_rows<E, std::void_t<decltype(E::kRowStores)>> : std::integral_constant<bool, E::kRowStores> {};
+
+// Staged epilogues with `static constexpr bool kSwizzledBox = true` have a tensor map with 64-byte
+// swizzle: the 16-byte pieces of a row go to banks by address alone, without the selects of the
+// plain box (their launches take kSmemBytesSwizzled).
+template <class E, class = void>
+struct epi_swizzled : std::false_type {};
+template <class E>
+struct epi_swizzled<E, std::void_t<decltype(E::kSwizzledBox)>> : std::integral_constant<bool, E::kSwizzledBox> {};
+
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
-__device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
 
 // Schedules with `static constexpr bool kOwnOperands = true` place their operands themselves
 // (other majors, 16-bit types, tensor maps or k-blocks than the plain GEMM's):
 //   issue_loads_pair(ti, kb, crank, sA, sB, bar)  this CTA's loads of one k-block, kStageBytes in all
-//   idesc(ti), a_desc(ti, addr, k), b_desc(ti, addr, k)  the MMA descriptors of k-step k of a stage
+// Their epilogues tell by rows_left(ti, row0) whether any output row follows row0.
+//   half_n(ti, h)          columns of half h that the tile needs (a multiple of 32, 0: none): the
+//                          last column block's MMAs are as narrow as its columns allow.  Each CTA
+//                          holds half_n / 2 rows of B, the leader's first
+//   idesc(ti, n), a_desc(ti, addr, k), b_desc(ti, addr, k)  the MMA descriptors of k-step k of a stage
+// and, with `static constexpr bool kLanes = true`,
 //   lane_skip(ti, kb, skip)  true: this k-block leaves the TMEM lanes set in skip[8] alone
 template <class S, class = void>
 struct sched_own : std::false_type {};
 template <class S>
 struct sched_own<S, std::void_t<decltype(S::kOwnOperands)>> : std::integral_constant<bool, S::kOwnOperands> {};
+// Dynamic schedules with `static constexpr bool kTileAhead = true` start with tile pair_id (their
+// counter starts at the number of pairs) and fetch each further index one tile ahead.
+template <class S, class = void>
+struct sched_ahead : std::false_type {};
+template <class S>
+struct sched_ahead<S, std::void_t<decltype(S::kTileAhead)>> : std::integral_constant<bool, S::kTileAhead> {};
+// `static constexpr bool kDependent = true`: the kernel may start before the one that it follows
+// has ended, and waits for it once its own set-up is done.
+template <class S, class = void>
+struct sched_dependent : std::false_type {};
+template <class S>
+struct sched_dependent<S, std::void_t<decltype(S::kDependent)>> : std::integral_constant<bool, S::kDependent> {};
+template <class S, class = void>
+struct sched_lanes : std::false_type {};
+template <class S>
+struct sched_lanes<S, std::void_t<decltype(S::kLanes)>> : std::integral_constant<bool, S::kLanes> {};
 
-// Epilogues with `static constexpr bool kGated = true` (NH = 2) get columns c of both halves at
-// once: gate(ti, row, c, lo, hi) combines 32 columns of half 0 and half 1 into hi, which is then
-// stored like one half's columns.
+// Epilogues with `static constexpr bool kGated = true` get two products side by side: NH = 2
+// column halves 0 and 1, NH = 1 accumulator columns 0..127 (the leader's rows of B) and 128..255
+// (the peer's).  gate(ti, row, c, lo, hi) combines 32 columns of both into hi, which is then
+// stored as columns c .. c+31 of the tile.
 template <class E, class = void>
 struct epi_gated : std::false_type {};
 template <class E>
@@ -314,6 +357,8 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
   cluster_sync();  // peer barriers initialised before any remote arrive / TMA completion
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // Launched over the end of the kernel before (programmatic launch): its results from here on.
+  if constexpr (sched_dependent<Sched>::value) ptx::griddep_wait();
   const int ntiles = sched.num_tiles();
   // the leader's queue-empty barriers and the peer's queue (leader writes it)
   const uint32_t tq_empty_leader = map_to(ptx::smem_u32(&tq_empty[0]), 0);
@@ -350,6 +395,7 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
         pol_a = lopt.l2hint == 1 ? keep : stream;
         pol_b = lopt.l2hint == 1 ? stream : keep;
       }
+      int ahead = pair_id;  // schedules with kTileAhead: the tile taken while the one before was loaded
       for (int t = pair_id; !*abort_flag; t += npairs) {
         if constexpr (kDyn) {
           if (leader) {
@@ -358,7 +404,12 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
               *abort_flag = 1;
               break;
             }
-            t = sched.next_tile();
+            if constexpr (sched_ahead<Sched>::value) {
+              t = ahead;
+              if (t < ntiles) ahead = sched.next_tile();
+            } else {
+              t = sched.next_tile();
+            }
             const int v = t < ntiles ? t : -1;
             tq[qslot] = v;
             st_cluster_u32(tq_peer + qslot * 4, v);
@@ -459,16 +510,21 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
         }
         ptx::tc_fence_after();
         const uint32_t d = tmem + acc * NH * BN2;
-        // k-step kb's MMAs for column halves [h0, h1) from the stage that holds it
-        auto issue = [&](int st, int kb, int h0, int h1) {
+        // k-step kb's MMAs for column halves [h0, h1) from the stage that holds it.  The
+        // lane-masked form is a loop of its own: beside it in one loop, the plain MMAs were
+        // issued too slowly to keep the tensor cores busy.
+        auto issue_mma = [&](auto lanes, const uint32_t* skip, int st, int kb, int h0, int h1) {
           const uint32_t a0 = ptx::smem_u32(sA + st * kABytes);
           const uint32_t b0 = ptx::smem_u32(sB + st * NH * kBBytes);
-          uint32_t idesc = idesc0;
-          uint32_t skip[8];
-          bool lanes = false;
-          if constexpr (sched_own<Sched>::value) {
-            idesc = sched.idesc(ti);
-            lanes = sched.lane_skip(ti, kb, skip);
+          uint32_t idesc[NH];
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            idesc[h] = idesc0;
+            if constexpr (sched_own<Sched>::value) {
+              const int n = sched.half_n(ti, h);
+              idesc[h] = sched.idesc(ti, n);
+              if (n == 0) h1 = h1 < h ? h1 : h;
+            }
           }
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
@@ -481,11 +537,21 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
               uint64_t bd;
               if constexpr (sched_own<Sched>::value) bd = sched.b_desc(ti, b0 + h * kBBytes, k);
               else bd = ptx::sdesc_kmajor_sw128(b0 + h * kBBytes + k * 32);
-              if (sched_own<Sched>::value && lanes) mma_pair_lanes(d + h * BN2, ad, bd, idesc, 1u, skip);
-              else if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc, (kb > ti.kb0 || k > 0) ? 1u : 0u);
-              else mma_pair(d + h * BN2, ad, bd, idesc, (kb > ti.kb0 || k > 0) ? 1u : 0u);
+              if constexpr (decltype(lanes)::value) mma_pair_lanes(d + h * BN2, ad, bd, idesc[h], 1u, skip);
+              else if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc[h], (kb > ti.kb0 || k > 0) ? 1u : 0u);
+              else mma_pair(d + h * BN2, ad, bd, idesc[h], (kb > ti.kb0 || k > 0) ? 1u : 0u);
             }
           }
+        };
+        auto issue = [&](int st, int kb, int h0, int h1) {
+          if constexpr (sched_lanes<Sched>::value) {
+            uint32_t skip[8];
+            if (sched.lane_skip(ti, kb, skip)) {
+              issue_mma(std::true_type{}, skip, st, kb, h0, h1);
+              return;
+            }
+          }
+          issue_mma(std::false_type{}, nullptr, st, kb, h0, h1);
         };
         auto release = [&](int st) {
           const uint32_t e_own = ptx::smem_u32(&empty[st]);
@@ -579,14 +645,18 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
     // SM over Cf::threads(kCommWarps) threads, 1 CTA per SM)
     constexpr int kRegs = 65536 / Cf::threads(Sched::kCommWarps);
     constexpr int kW0 = kRegs >= 200 ? 128 : (kRegs >= 136 ? 64 : 32);
-    constexpr int kW = kW0 < kSeg ? kW0 : kSeg;
+    // (64 where the schedule's and epilogue's own state needs registers too)
+    constexpr int kW1 = sched_own<Sched>::value && kW0 > 64 ? 64 : kW0;
+    constexpr int kW = kW1 < kSeg ? kW1 : kSeg;
     const int q = warp & 3;
     const int part = NH == 1 ? 0 : ((int)warp - 2) / 4;
     const int row = q * 32 + lane;
-    // Staged stores: this warp's two 32 x 32 bf16 boxes, used in turn; the TMA store that
+    // Staged stores: this warp's 32 x 32 16-bit boxes, used in turn; the TMA store that
     // read a box must have finished reading it before the box is written again.
     constexpr bool kStaged = epi_staged<Epi>::value;
-    uint8_t* my_boxes = smem + S * Cf::kStageBytes + 256 + ((int)warp - 2) * 2 * Cf::kBoxBytes;
+    constexpr bool kSwz = epi_swizzled<Epi>::value;
+    constexpr int kBoxes = kSwz ? Cf::kSwzBoxes : 2;
+    uint8_t* my_boxes = smem + S * Cf::kStageBytes + (kSwz ? 512 : 256) + ((int)warp - 2) * kBoxes * Cf::kBoxBytes;
     uint32_t box_turn = 0;
     const uint32_t tempty_leader0 = map_to(ptx::smem_u32(&tempty[0]), 0);
     const uint32_t tempty_leader1 = map_to(ptx::smem_u32(&tempty[1]), 0);
@@ -618,21 +688,34 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
       // from the registers
       auto put = [&](const uint32_t* ri, int col) {
         if constexpr (kStaged) {
-          if (epi.staged()) {
-            uint8_t* box = my_boxes + (box_turn & 1) * Cf::kBoxBytes;
+          if (epi_rows<Epi>::value || epi.staged()) {
+            uint8_t* box = my_boxes + (box_turn & (kBoxes - 1)) * Cf::kBoxBytes;
             ++box_turn;
-            if (lane == 0) bulk_wait_read_1();  // the store issued from this box two chunks ago
+            if (lane == 0) bulk_wait_read<kBoxes - 1>();  // the store issued from this box kBoxes chunks ago
             __syncwarp();
             uint4 v[4];
             epi.pack(ri, v);
             // row `lane` of the box (64 bytes); the 16-byte pieces are written in an
             // order rotated by lane/2, so each group of 8 lanes covers all 32 banks
             const uint32_t rowaddr = ptx::smem_u32(box) + lane * 64;
+            if constexpr (kSwz) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int cj = (j + (int)(lane >> 1)) & 3;
-              const uint4 w = cj == 0 ? v[0] : cj == 1 ? v[1] : cj == 2 ? v[2] : v[3];
-              st_shared_v4(rowaddr + cj * 16, w);
+              for (int j = 0; j < 4; ++j) st_shared_v4(rowaddr + ((j ^ ((lane >> 1) & 3)) * 16), v[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int cj = (j + (int)(lane >> 1)) & 3;
+                const uint4 w = cj == 0 ? v[0] : cj == 1 ? v[1] : cj == 2 ? v[2] : v[3];
+                st_shared_v4(rowaddr + cj * 16, w);
+              }
+            }
+            if constexpr (epi_rows<Epi>::value) {
+              if (!epi.staged()) {
+                __syncwarp();
+                epi.store_rows(ti, q * 32, col, reinterpret_cast<const uint16_t*>(box), (int)lane);
+                __syncwarp();
+                return;
+              }
             }
             ptx::fence_proxy_async_smem();
             __syncwarp();
@@ -647,34 +730,57 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
         epi.store(ti, row, col, ri);
       };
       if constexpr (epi_gated<Epi>::value) {
-        // This warp's first 32 columns of both halves, then the other 96 of half 0 into registers
-        // (all 128 at once would spill), which frees half 0 for the next tile's first k-steps
-        // after a quarter of the drain; half 1 follows 32 columns at a time.
-        static_assert(!epi_gated<Epi>::value || (NH == 2 && !Epi::kNeedsTileDone), "gated epilogue: 256 x 512 tiles");
-        uint32_t lo[kSeg - 32], hi[32];
-        const int c0 = part * kSeg;
-        ptx::tmem_ld32(tbase + c0, lo);
-        ptx::tmem_ld32(tbase + BN2 + c0, hi);
-        ptx::tmem_ld_wait();
-        epi.gate(ti, row, c0, lo, hi);
-        put(hi, c0);
-#pragma unroll
-        for (int i = 1; i < kSeg / 32; ++i) ptx::tmem_ld32(tbase + c0 + 32 * i, lo + 32 * (i - 1));
-        ptx::tmem_ld_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(tempty_leader0);
-#pragma unroll
-        for (int i = 1; i < kSeg / 32; ++i) {
-          ptx::tmem_ld32(tbase + BN2 + c0 + 32 * i, hi);
-          ptx::tmem_ld_wait();
-          if (i + 1 == kSeg / 32) {
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(tempty_leader1);
+        static_assert(!epi_gated<Epi>::value || !Epi::kNeedsTileDone, "gated epilogue: no tile-done hook");
+        if constexpr (NH == 1) {
+          // columns c of half 0 and half 1 = accumulator columns c and 128 + c
+          // (n / 2 + c for a tile of n columns)
+          const uint32_t free_bar = acc ? tempty_leader1 : tempty_leader0;
+          const int n2 = sched.half_n(ti, 0) / 2;
+#pragma unroll 1
+          for (int c = 0; c < n2; c += 32) {
+            uint32_t lo[32], hi[32];
+            ptx::tmem_ld32(tbase + c, lo);
+            ptx::tmem_ld32(tbase + n2 + c, hi);
+            ptx::tmem_ld_wait();
+            if (c + 32 >= n2) {
+              ptx::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_cluster(free_bar);
+            }
+            if (epi.rows_left(ti, q * 32) <= 0) continue;
+            epi.gate(ti, row, c, lo, hi);
+            put(hi, c);
           }
-          epi.gate(ti, row, c0 + 32 * i, lo + 32 * (i - 1), hi);
-          put(hi, c0 + 32 * i);
+        } else {
+          // This warp's first 32 columns of both halves, then the other 96 of half 0 into registers
+          // (all 128 at once would spill), which frees half 0 for the next tile's first k-steps
+          // after a quarter of the drain; half 1 follows 32 columns at a time.
+          constexpr int kSeg2 = BN2 / 2;
+          uint32_t lo[kSeg2 - 32], hi[32];
+          const int c0 = part * kSeg2;
+          ptx::tmem_ld32(tbase + c0, lo);
+          ptx::tmem_ld32(tbase + BN2 + c0, hi);
+          ptx::tmem_ld_wait();
+          epi.gate(ti, row, c0, lo, hi);
+          put(hi, c0);
+#pragma unroll
+          for (int i = 1; i < kSeg2 / 32; ++i) ptx::tmem_ld32(tbase + c0 + 32 * i, lo + 32 * (i - 1));
+          ptx::tmem_ld_wait();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_cluster(tempty_leader0);
+#pragma unroll
+          for (int i = 1; i < kSeg2 / 32; ++i) {
+            ptx::tmem_ld32(tbase + BN2 + c0 + 32 * i, hi);
+            ptx::tmem_ld_wait();
+            if (i + 1 == kSeg2 / 32) {
+              ptx::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) arrive_cluster(tempty_leader1);
+            }
+            epi.gate(ti, row, c0 + 32 * i, lo + 32 * (i - 1), hi);
+            put(hi, c0 + 32 * i);
+          }
         }
       } else {
 #pragma unroll 1
@@ -686,9 +792,14 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
             // kW columns: every TMEM load issued before one wait (each wait is a round trip)
             const int col0 = h * BN2 + part * kSeg + c;
             uint32_t r[kW];
+            bool needed = true;  // not past the columns that the tile has
+            if constexpr (sched_own<Sched>::value)
+              needed = part * kSeg + c < sched.half_n(ti, h) && epi.rows_left(ti, q * 32) > 0;
+            if (needed) {
 #pragma unroll
-            for (int i = 0; i < kW / 32; ++i) ptx::tmem_ld32(tbase + col0 + 32 * i, r + 32 * i);
-            ptx::tmem_ld_wait();
+              for (int i = 0; i < kW / 32; ++i) ptx::tmem_ld32(tbase + col0 + 32 * i, r + 32 * i);
+              ptx::tmem_ld_wait();
+            }
             // Epilogues that publish finished tiles free the last half only after tile_done
             // (below); half 0 of a 512-column accumulator can go back at once, because the
             // next tile's epilogue cannot start before half 1 is free.
@@ -699,6 +810,7 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
                 if (lane == 0) arrive_cluster(free_bar);
               }
             }
+            if (!needed) continue;
 #pragma unroll
             for (int i = 0; i < kW / 32; ++i) put(r + 32 * i, col0 + 32 * i);
           }

@@ -25,23 +25,30 @@ namespace split {
 constexpr int kRows = 128;              // rows of a tile (TMEM lanes)
 constexpr int kThreads = 192;
 constexpr int kMaxSplit = 8;            // portable cluster size
-constexpr int kMaxCols = 128;           // columns of one weight per tile
+constexpr int kMaxCols = 256;           // columns of all weights per tile (the MMA's N)
 constexpr int kMaxStages = 12;
-constexpr uint32_t kXBytes = kRows * BK * 2;
 constexpr uint32_t kBarBytes = (2 * kMaxStages + 2) * 8 + 16;
 
 struct Shape {
   int T, N, K;   // rows of X, rows of each W, depth
   int bn;        // columns per tile and weight: a multiple of 16
+  int mblocks;   // tiles of 128 rows
   int xrows;     // rows of an X box: min(128, T rounded up to 8)
+  int group;     // k-blocks per ring stage
   int stages;
 };
 
-__host__ __device__ constexpr uint32_t stage_bytes(int accs, int bn) { return kXBytes + accs * bn * BK * 2; }
+__host__ __device__ constexpr uint32_t x_bytes(int xrows) { return xrows * BK * 2; }        // of one k-block
+__host__ __device__ constexpr uint32_t w_bytes(int accs, int bn) { return accs * bn * BK * 2; }
 // floats between two rows of a partial: + 4 keeps the 16-byte writes of 8 lanes on 32 banks
 __host__ __device__ constexpr int pitch(int accs, int bn) { return accs * bn + 4; }
-__host__ __device__ constexpr uint32_t ring_bytes(int accs, int bn, int stages, int rows) {
-  const uint32_t ring = stages * stage_bytes(accs, bn), part = rows * pitch(accs, bn) * 4;
+// The ring (X of all stages, then W), or the partial that takes its place.  The MMA reads 128
+// rows of X whatever xrows is: the rows behind an X box are other data of the ring, and their
+// lanes are never read; the last box has 16 KB of ring behind its start.
+__host__ __device__ constexpr uint32_t ring_bytes(int accs, int bn, int xrows, int group, int stages, int rows) {
+  uint32_t ring = stages * group * (x_bytes(xrows) + w_bytes(accs, bn));
+  const uint32_t reach = (stages * group - 1) * x_bytes(xrows) + kRows * BK * 2, part = rows * pitch(accs, bn) * 4;
+  if (reach > ring) ring = reach;
   return ((ring > part ? ring : part) + 127) / 128 * 128;
 }
 __host__ __device__ constexpr uint32_t tmem_cols(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256; }
@@ -72,25 +79,51 @@ __device__ __forceinline__ void store4_16(uint16_t* row, int col, int N, const f
   }
 }
 
-// Op: kAccs (weights multiplied side by side), fmt() (16-bit type), and
+// Op: kAccs (weights multiplied side by side) and
 //   prepare(smem_extra, t0, ...)   by all threads before the pipeline starts
+//   loads(kb, t0, n0, x, w, bar)   the loads of k-block kb (x_bytes + w_bytes in all)
+//   idesc(n), x_desc(addr, k), w_desc(addr, k)  the MMA descriptors of k-step k of a k-block
+//   depth()                        k-blocks
 //   extra_blocks(c, S, e0, e1)     this CTA's further k-blocks after the weights'
 //   extra_wait()                   by the producer before the first of them
-//   extra_loads(e, sh, t0, n0, sX, sW, bar)   loads of one (stage_tx() bytes, as a weight block)
-//   extra_mma(e, d, xs, ws, idesc)            its MMAs
+//   extra_loads(e, t0, n0, x, w, bar)         loads of one (as many bytes as a k-block's)
+//   extra_mma(e, d, x, w, idesc)              its MMAs
 //   emit(row, col, v)              v[i][4]: four columns of weight i of one valid row
 //   finish()                       by all threads, last
+// The K-major operands and no further k-blocks: the base of most Ops.
+struct PlainOp {
+  int type;                 // 0 = f16, 1 = bf16
+  const CUtensorMap* tmX;   // set by the kernel
+  const CUtensorMap* tmW;
+  __device__ void prepare(uint8_t*, int, ErrorRecord*) {}
+  __device__ void prefetch_maps() const {
+    ptx::prefetch_tmap(tmX);
+    ptx::prefetch_tmap(tmW);
+  }
+  __device__ uint32_t idesc(int n) const { return ptx::idesc_f16_f32(kRows, n, type, 0, 0); }
+  __device__ uint64_t x_desc(uint32_t x, int k) const { return ptx::sdesc_kmajor_sw128(x + k * 32); }
+  __device__ uint64_t w_desc(uint32_t w, int k) const { return ptx::sdesc_kmajor_sw128(w + k * 32); }
+  __device__ void loads(int kb, int t0, int n0, uint8_t* x, uint8_t* w, uint64_t* bar) const {
+    ptx::tma_load_2d(w, tmW, bar, kb * BK, n0);
+    ptx::tma_load_2d(x, tmX, bar, kb * BK, t0);
+  }
+  __device__ void extra_blocks(int, int, int& e0, int& e1) const { e0 = e1 = 0; }
+  __device__ void extra_wait() const {}
+  __device__ void extra_loads(int, int, int, uint8_t*, uint8_t*, uint64_t*) const {}
+  __device__ void extra_mma(int, uint32_t, uint32_t, uint32_t, uint32_t) const {}
+  __device__ void finish() const {}
+};
+
 template <class Op>
-__device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtensorMap* tmW0, const CUtensorMap* tmW1,
-                                           const Shape& sh, Op& op, ErrorRecord* err, uint64_t timeout_ns) {
+__device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord* err, uint64_t timeout_ns) {
   constexpr int A = Op::kAccs;
   extern __shared__ uint8_t split_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(split_smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = sh.stages;
-  const uint32_t wbytes = sh.bn * BK * 2;
+  const int stages = sh.stages, group = sh.group;
+  const uint32_t xb = x_bytes(sh.xrows), wb = w_bytes(A, sh.bn);
   uint8_t* sX = smem;
-  uint8_t* sW = smem + stages * kXBytes;  // per stage: A consecutive blocks of wbytes
-  uint8_t* after = smem + ring_bytes(A, sh.bn, stages, kRows);
+  uint8_t* sW = smem + stages * group * xb;  // per k-block: bn rows of each weight
+  uint8_t* after = smem + ring_bytes(A, sh.bn, sh.xrows, group, stages, kRows);
   uint64_t* full = reinterpret_cast<uint64_t*>(after);
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
@@ -104,9 +137,10 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
   const int S = (int)cluster_size();
   const int c = (int)pair::cta_rank();
   const int n0 = (int)(blockIdx.x / S) * sh.bn;
-  const int t0 = (int)blockIdx.y * kRows;
+  const int t0 = (int)blockIdx.y % sh.mblocks * kRows;  // blockIdx.y / mblocks: the Op's further index
   const int rows = min(kRows, sh.T - t0);
-  const uint32_t ncols = tmem_cols(A * sh.bn);
+  const int ncol = A * sh.bn;
+  const uint32_t tcols = tmem_cols(ncol);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -117,11 +151,10 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
-    ptx::prefetch_tmap(tmX);
-    ptx::prefetch_tmap(tmW0);
+    op.prefetch_maps();
   }
   if (warp == 1) {
-    ptx::tmem_alloc(tmem_slot, ncols);
+    ptx::tmem_alloc(tmem_slot, tcols);
     ptx::tmem_relinquish();
   }
   op.prepare(after + kBarBytes, t0, err);
@@ -129,35 +162,36 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int nkb = (sh.K + BK - 1) / BK;
-  const int kb0 = (int)((long long)nkb * c / S), kb1 = (int)((long long)nkb * (c + 1) / S);
+  const int nkb = op.depth();
+  const int kb0 = (int)((long long)nkb * c / S), nk = (int)((long long)nkb * (c + 1) / S) - kb0;
   int e0, e1;
   op.extra_blocks(c, S, e0, e1);
-  const int steps = (kb1 - kb0) + (e1 - e0);  // >= 1: the host takes S <= nkb
+  const int blocks = nk + (e1 - e0);  // nk >= 1: the host takes S <= nkb
+  const int steps = (blocks + group - 1) / group;
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t tx = sh.xrows * BK * 2 + A * wbytes;
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
       for (int i = 0; i < steps; ++i) {
-        if (i == kb1 - kb0) op.extra_wait();
         if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
           if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
           *abort_flag = 1;
           break;
         }
-        ptx::mbar_arrive_expect_tx(&full[stage], tx);
-        uint8_t* x = sX + stage * kXBytes;
-        uint8_t* w = sW + stage * A * wbytes;
-        if (i < kb1 - kb0) {
-          const int kx = (kb0 + i) * BK;
-          ptx::tma_load_2d(x, tmX, &full[stage], kx, t0);
-          ptx::tma_load_2d(w, tmW0, &full[stage], kx, n0);
-          if constexpr (A == 2) ptx::tma_load_2d(w + wbytes, tmW1, &full[stage], kx, n0);
-        } else {
-          op.extra_loads(e0 + i - (kb1 - kb0), t0, n0, x, w, &full[stage]);
+        const int b0 = i * group, nb = min(group, blocks - b0);
+        ptx::mbar_arrive_expect_tx(&full[stage], nb * (xb + wb));
+        for (int j = 0; j < nb; ++j) {
+          const int b = b0 + j;
+          uint8_t* x = sX + (stage * group + j) * xb;
+          uint8_t* w = sW + (stage * group + j) * wb;
+          if (b < nk) {
+            op.loads(kb0 + b, t0, n0, x, w, &full[stage]);
+          } else {
+            if (b == nk) op.extra_wait();
+            op.extra_loads(e0 + b - nk, t0, n0, x, w, &full[stage]);
+          }
         }
         issued = i + 1;
         if (++stage == stages) {
@@ -174,7 +208,7 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = ptx::idesc_f16_f32(kRows, sh.bn, op.fmt(), 0, 0);
+      const uint32_t idesc = op.idesc(ncol);
       int stage = 0;
       uint32_t phase = 0;
       int i = 0;
@@ -185,19 +219,17 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
           break;
         }
         ptx::tc_fence_after();
-        const uint32_t x = ptx::smem_u32(sX + stage * kXBytes);
-        const uint32_t w = ptx::smem_u32(sW + stage * A * wbytes);
-        if (i < kb1 - kb0) {
+        const int b0 = i * group, nb = min(group, blocks - b0);
+        for (int j = 0; j < nb; ++j) {
+          const uint32_t x = ptx::smem_u32(sX + (stage * group + j) * xb);
+          const uint32_t w = ptx::smem_u32(sW + (stage * group + j) * wb);
+          if (b0 + j < nk) {
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t ad = ptx::sdesc_kmajor_sw128(x + k * 32);
-#pragma unroll
-            for (int a = 0; a < A; ++a)
-              ptx::mma_f16_ss(tmem + a * sh.bn, ad, ptx::sdesc_kmajor_sw128(w + a * wbytes + k * 32), idesc,
-                              (i > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k)
+              ptx::mma_f16_ss(tmem, op.x_desc(x, k), op.w_desc(w, k), idesc, (b0 + j > 0 || k > 0) ? 1u : 0u);
+          } else {
+            op.extra_mma(e0 + b0 + j - nk, tmem, x, w, idesc);
           }
-        } else {
-          op.extra_mma(e0 + i - (kb1 - kb0), tmem, x, w, idesc);
         }
         ptx::mma_commit(&empty[stage]);
         if (++stage == stages) {
@@ -223,7 +255,7 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
       ptx::tc_fence_after();
       const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16);
       float* dst = part + row * pitch(A, sh.bn);
-      for (int col = 0; col < A * sh.bn; col += 16) {
+      for (int col = 0; col < ncol; col += 16) {
         uint32_t r[16];
         ptx::tmem_ld16(tbase + col, r);
         ptx::tmem_ld_wait();
@@ -274,7 +306,7 @@ __device__ __forceinline__ void split_core(const CUtensorMap* tmX, const CUtenso
   pair::cluster_sync();  // no CTA leaves while its partial is being read
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, ncols);
+    ptx::tmem_dealloc(tmem, tcols);
   }
 }
 

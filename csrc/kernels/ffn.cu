@@ -53,7 +53,9 @@ struct GatedMaps {
   CUtensorMap x, g, u, h;
 };
 
+template <int NH>
 struct GatedSched {
+  static constexpr int kCols = NH * pair::BN2 / 2;  // columns of h per tile
   static constexpr int kCommWarps = 0;
   static constexpr bool kOwnOperands = true;
   int T, I, H;
@@ -66,7 +68,7 @@ struct GatedSched {
     raster(t, num_m, num_n, group_m, mb, nb);
     TileInfo ti;
     ti.m0 = mb * 2 * BM;
-    ti.n0 = nb * pair::BN2;
+    ti.n0 = nb * kCols;
     ti.a_row = ti.m0;
     ti.b_row = ti.n0;
     ti.kb0 = 0;
@@ -78,13 +80,22 @@ struct GatedSched {
   __device__ bool producer_wait(const TileInfo&, int, uint64_t, volatile int*, ErrorRecord*) const { return true; }
   __device__ void issue_loads_pair(const TileInfo& ti, int kb, int crank, uint8_t* sA, uint8_t* sB, uint32_t bar) const {
     pair::tma_load_2d_pair(sA, &maps->x, bar, kb * BK, ti.a_row + crank * BM);
-    pair::tma_load_2d_pair(sB, &maps->g, bar, kb * BK, ti.b_row + crank * BM);
-    pair::tma_load_2d_pair(sB + pair::kBBytes, &maps->u, bar, kb * BK, ti.b_row + crank * BM);
+    if constexpr (NH == 2) {
+      const int n = ti.b_row + crank * half_n(ti, 0) / 2;
+      pair::tma_load_2d_pair(sB, &maps->g, bar, kb * BK, n);
+      pair::tma_load_2d_pair(sB + pair::kBBytes, &maps->u, bar, kb * BK, n);
+    } else {
+      pair::tma_load_2d_pair(sB, crank == 0 ? &maps->g : &maps->u, bar, kb * BK, ti.b_row);
+    }
   }
-  __device__ uint32_t idesc(const TileInfo&) const { return ptx::idesc_f16_f32(2 * BM, pair::BN2, fmt, 0, 0); }
+  // NH = 2: the tile's columns of each weight; NH = 1: of both
+  __device__ int half_n(const TileInfo& ti, int) const {
+    const int left = I - ti.n0;
+    return NH == 2 ? min(pair::BN2, (left + 31) / 32 * 32) : 2 * min(pair::BN2 / 2, (left + 31) / 32 * 32);
+  }
+  __device__ uint32_t idesc(const TileInfo&, int n) const { return ptx::idesc_f16_f32(2 * BM, n, fmt, 0, 0); }
   __device__ uint64_t a_desc(const TileInfo&, uint32_t a, int k) const { return ptx::sdesc_kmajor_sw128(a + k * 32); }
   __device__ uint64_t b_desc(const TileInfo&, uint32_t b, int k) const { return ptx::sdesc_kmajor_sw128(b + k * 32); }
-  __device__ bool lane_skip(const TileInfo&, int, uint32_t*) const { return false; }
 };
 
 struct GatedEpi : Out16Epi {
@@ -99,6 +110,7 @@ struct GatedEpi : Out16Epi {
   }
   __device__ __forceinline__ void gate(const TileInfo& ti, int row, int c, const uint32_t* lo, uint32_t* hi) const {
     const int t = ti.m0 + row, i = ti.n0 + c;
+    if (ti.m0 + (row & ~31) >= M) return;  // none of the warp's rows exists
     if (saved != nullptr && t < M) {
       float* g = saved + saved_at(t, i, N);
       float* u = g + saved_plane(M, N);
@@ -116,28 +128,28 @@ struct GatedEpi : Out16Epi {
   }
 };
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<2>::kThreads, 1)
-    k_gated_pair(const __grid_constant__ GatedMaps maps, GatedSched sched, GatedEpi epi, ErrorRecord* err,
+template <int NH>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::kThreads, 1)
+    k_gated_pair(const __grid_constant__ GatedMaps maps, GatedSched<NH> sched, GatedEpi epi, ErrorRecord* err,
                  uint64_t timeout_ns) {
   sched.maps = &maps;
   epi.tmC = &maps.h;
-  pair::gemm_core_pair<2>(&maps.x, &maps.g, sched, epi, err, timeout_ns, -1);
+  pair::gemm_core_pair<NH>(&maps.x, &maps.g, sched, epi, err, timeout_ns, -1);
 }
 
 // ---- forward for few rows ------------------------------------------------------------------
-struct GatedSplitOp {
+struct GatedSplitOp : split::PlainOp {
   static constexpr int kAccs = 2;
+  const CUtensorMap* tmU;  // set by the kernel
   uint16_t* h;
   long long ldh;
-  int T, I, kind, type, vec;
+  int T, H, I, kind, vec, bn;
   float* saved;
-  __device__ int fmt() const { return type; }
-  __device__ void prepare(uint8_t*, int, ErrorRecord*) {}
-  __device__ void extra_blocks(int, int, int& e0, int& e1) const { e0 = e1 = 0; }
-  __device__ void extra_wait() const {}
-  __device__ void extra_loads(int, int, int, void*, void*, uint64_t*) const {}
-  __device__ void extra_mma(int, uint32_t, uint32_t, uint32_t, uint32_t) const {}
-  __device__ void finish() const {}
+  __device__ int depth() const { return (H + BK - 1) / BK; }
+  __device__ void loads(int kb, int t0, int n0, uint8_t* x, uint8_t* w, uint64_t* bar) const {
+    PlainOp::loads(kb, t0, n0, x, w, bar);
+    ptx::tma_load_2d(w + bn * BK * 2, tmU, bar, kb * BK, n0);
+  }
   __device__ __forceinline__ void emit(int t, int i, const float (*v)[4]) const {
     if (saved != nullptr && i < saved_cols(I)) {
       float* g = saved + saved_at(t, i, I);
@@ -155,85 +167,136 @@ __global__ void __launch_bounds__(split::kThreads, 1)
     k_gated_split(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG,
                   const __grid_constant__ CUtensorMap tmU, split::Shape sh, GatedSplitOp op, ErrorRecord* err,
                   uint64_t timeout_ns) {
-  split::split_core(&tmX, &tmG, &tmU, sh, op, err, timeout_ns);
+  op.tmX = &tmX;
+  op.tmW = &tmG;
+  op.tmU = &tmU;
+  split::split_core(sh, op, err, timeout_ns);
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// One warp per 32 rows x 16 columns: a lane is a row (as in the saved layout), so g and u come
-// as 512-byte warp loads and dh, dg and du as whole 32-byte sectors of a row.
+// One block per 32 rows x 128 columns.  In the saved layout a lane is a row, so g and u come as
+// 512-byte warp loads; dh, dg and du pass through shared memory, so that their global accesses
+// are whole 256-byte row pieces too.  Bound by its 14 bytes per element (saved 8, dh 2, dg and
+// du 4).  The first block also sets the tile counter of k_gated_bwd.
+constexpr int kGradCols = 128;
+constexpr int kGradPitch = kGradCols + 8;  // 16-bit words: 16-byte accesses of 8 rows on 32 banks
+
 __global__ void __launch_bounds__(256)
     k_gate_grad(const uint16_t* __restrict__ dh, long long lddh, const float* __restrict__ saved,
-                uint16_t* __restrict__ dgu, int T, int I, int Ip, int kind, int fmt, int vec) {
-  const int cb = saved_cols(I) / 16;
-  const long long blocks = (long long)((T + 31) / 32) * cb;
-  const int lane = threadIdx.x & 31;
+                uint16_t* __restrict__ dgu, int T, int I, int Ip, int kind, int fmt, int vec, unsigned int* counter,
+                unsigned int first_tile) {
+  __shared__ alignas(16) uint16_t sd[32 * kGradPitch], so[2][32 * kGradPitch];
+  ptx::griddep_launch();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = first_tile;
+  const int i0 = blockIdx.x * kGradCols;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t plane = saved_plane(T, I), out_plane = (size_t)T * Ip;
-  for (long long b = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; b < blocks;
-       b += (long long)gridDim.x * (blockDim.x / 32)) {
-    const int t = (int)(b / cb) * 32 + lane, i = (int)(b % cb) * 16;
-    if (t >= T) continue;
-    const uint16_t* dp = dh + (size_t)t * lddh + i;
-    uint16_t d[16];
-    if (vec && i + 16 <= I) {
-      *reinterpret_cast<uint4*>(d) = ptx::ld_v4_nc(dp);
-      *reinterpret_cast<uint4*>(d + 8) = ptx::ld_v4_nc(dp + 8);
-    } else {
+  for (int tb = blockIdx.y; tb < (T + 31) / 32; tb += gridDim.y) {
+    const int t0 = tb * 32, rows = min(32, T - t0);
+    const int t = t0 + lane, i = i0 + warp * 16;
+    const bool work = lane < rows && i < saved_cols(I);
+    uint4 gv[4], uv[4];
+    if (work) {
+      const float* gp = saved + saved_at(t, i, I);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) d[j] = i + j < I ? dp[j] : (uint16_t)0;
-    }
-    const float* gp = saved + saved_at(t, i, I);
-    uint32_t og[8], ou[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint4 gv = ptx::ld_v4_nc(gp + 128 * j), uv = ptx::ld_v4_nc(gp + plane + 128 * j);
-      const float g[4] = {__uint_as_float(gv.x), __uint_as_float(gv.y), __uint_as_float(gv.z), __uint_as_float(gv.w)};
-      const float u[4] = {__uint_as_float(uv.x), __uint_as_float(uv.y), __uint_as_float(uv.z), __uint_as_float(uv.w)};
-      float a[4], e[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float dv = ptx::from_16(d[4 * j + k], fmt);
-        float slope;
-        a[k] = dv * act::value_grad(g[k], kind, &slope);
-        e[k] = dv * u[k] * slope;
+      for (int j = 0; j < 4; ++j) {
+        gv[j] = ptx::ld_v4_nc(gp + 128 * j);
+        uv[j] = ptx::ld_v4_nc(gp + plane + 128 * j);
       }
-      og[2 * j] = ptx::pack_16x2(e[0], e[1], fmt);
-      og[2 * j + 1] = ptx::pack_16x2(e[2], e[3], fmt);
-      ou[2 * j] = ptx::pack_16x2(a[0], a[1], fmt);
-      ou[2 * j + 1] = ptx::pack_16x2(a[2], a[3], fmt);
     }
-    uint16_t* p = dgu + (size_t)t * Ip + i;  // Ip % 64 == 0: the row holds all 16 columns
-    ptx::st_v4(p, make_uint4(og[0], og[1], og[2], og[3]));
-    ptx::st_v4(p + 8, make_uint4(og[4], og[5], og[6], og[7]));
-    ptx::st_v4(p + out_plane, make_uint4(ou[0], ou[1], ou[2], ou[3]));
-    ptx::st_v4(p + out_plane + 8, make_uint4(ou[4], ou[5], ou[6], ou[7]));
+    if (vec) {
+      for (int q = threadIdx.x; q < 32 * (kGradCols / 8); q += 256) {
+        const int r = q / (kGradCols / 8), col = q % (kGradCols / 8) * 8;
+        if (r >= rows || i0 + col >= I) continue;
+        const uint16_t* p = dh + (size_t)(t0 + r) * lddh + i0 + col;
+        uint16_t* d = sd + r * kGradPitch + col;
+        if (i0 + col + 8 <= I) {
+          *reinterpret_cast<uint4*>(d) = ptx::ld_v4_nc(p);
+        } else {
+          for (int k = 0; i0 + col + k < I; ++k) d[k] = p[k];
+        }
+      }
+    } else {
+#pragma unroll 8
+      for (int q = threadIdx.x; q < 32 * kGradCols; q += 256) {
+        const int r = q / kGradCols, col = q % kGradCols;
+        if (r < rows && i0 + col < I) sd[r * kGradPitch + col] = dh[(size_t)(t0 + r) * lddh + i0 + col];
+      }
+    }
+    __syncthreads();
+    if (work) {
+      const uint4* dp = reinterpret_cast<const uint4*>(sd + lane * kGradPitch + warp * 16);
+      uint16_t d[16];
+      *reinterpret_cast<uint4*>(d) = dp[0];
+      *reinterpret_cast<uint4*>(d + 8) = dp[1];
+      uint32_t og[8], ou[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float g[4] = {__uint_as_float(gv[j].x), __uint_as_float(gv[j].y), __uint_as_float(gv[j].z), __uint_as_float(gv[j].w)};
+        const float u[4] = {__uint_as_float(uv[j].x), __uint_as_float(uv[j].y), __uint_as_float(uv[j].z), __uint_as_float(uv[j].w)};
+        float a[4], e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // columns past I (never read back) hold whatever the tile held before
+          const float dv = ptx::from_16(d[4 * j + k], fmt);
+          float slope;
+          a[k] = dv * act::value_grad(g[k], kind, &slope);
+          e[k] = dv * u[k] * slope;
+        }
+        og[2 * j] = ptx::pack_16x2(e[0], e[1], fmt);
+        og[2 * j + 1] = ptx::pack_16x2(e[2], e[3], fmt);
+        ou[2 * j] = ptx::pack_16x2(a[0], a[1], fmt);
+        ou[2 * j + 1] = ptx::pack_16x2(a[2], a[3], fmt);
+      }
+      uint4* pg = reinterpret_cast<uint4*>(so[0] + lane * kGradPitch + warp * 16);
+      uint4* pu = reinterpret_cast<uint4*>(so[1] + lane * kGradPitch + warp * 16);
+      pg[0] = make_uint4(og[0], og[1], og[2], og[3]);
+      pg[1] = make_uint4(og[4], og[5], og[6], og[7]);
+      pu[0] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+      pu[1] = make_uint4(ou[4], ou[5], ou[6], ou[7]);
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < 2 * 32 * (kGradCols / 8); q += 256) {
+      const int z = q / (32 * (kGradCols / 8)), r = q / (kGradCols / 8) % 32, col = q % (kGradCols / 8) * 8;
+      if (r < rows && i0 + col < saved_cols(I))  // saved_cols(I) <= Ip
+        ptx::st_v4(dgu + z * out_plane + (size_t)(t0 + r) * Ip + i0 + col,
+                   *reinterpret_cast<const uint4*>(so[z] + r * kGradPitch + col));
+    }
   }
 }
 
 struct BwdMaps {
   CUtensorMap d_rows;  // [2][T][I] dg, du: boxes of 128 rows x 64 columns (A of dx, K-major)
+  CUtensorMap d_split; // the same: boxes of as many rows as a split-K tile has
   CUtensorMap d_cols;  // the same: boxes of 64 rows x 64 columns (A of the weight gradients, M-major)
-  CUtensorMap wg, wu;  // [I][H]: boxes of 64 x 64 (B of dx, N-major)
+  CUtensorMap w[2];    // Wg, Wu [I][H]: boxes of 64 x 64 (B of dx, N-major)
   CUtensorMap x;       // [T][H]: boxes of 64 x 64 (B of the weight gradients, N-major)
   CUtensorMap dx, dwg, dwu;  // output boxes of 32 x 32
 };
 
-// TileInfo::aux: 0 dx, 1 dWg, 2 dWu.
+// The backward products' tiles on CTA pairs.  TileInfo::aux: 0 dx, 1 dWg, 2 dWu.  Tiles are taken
+// in order from a counter: the products' depths differ, and the deeper comes first.
+template <int NH>
 struct BwdSched {
   static constexpr int kCommWarps = 0;
   static constexpr bool kOwnOperands = true;
+  static constexpr bool kDynamic = true;
+  static constexpr bool kTileAhead = true;
+  static constexpr bool kDependent = true;
+  unsigned int* counter;
+  __device__ int next_tile() const { return (int)atomicAdd(counter, 1u); }
   int T, H, I;
-  int nx, nw;              // tiles of dx (0: not wanted) and of each weight gradient (0: not wanted)
-  int mx, mw, nn;          // 256-row m-blocks of dx and of a weight gradient; 512-column n-blocks
-  int x_first;             // dx's tiles first (the deeper product first, for a short last wave)
+  int nx, nw;              // tiles of dx (0: not wanted here) and of each weight gradient (the same)
+  int mx, mw, nn;          // 256-row m-blocks of dx and of a weight gradient; column blocks
+  int x_first;             // dx's tiles first
   int group_m;
   int fmt;
   const BwdMaps* maps;
-  __device__ int num_tiles() const { return nx + 2 * nw; }
+  __host__ __device__ int num_tiles() const { return nx + 2 * nw; }
   __device__ TileInfo tile(int t) const {
     TileInfo ti;
     int mb, nb;
     const bool is_x = x_first ? t < nx : t >= 2 * nw;
-    ti.kb0 = 0;
     if (is_x) {
       raster(x_first ? t : t - 2 * nw, mx, nn, group_m, mb, nb);
       ti.aux = 0;
@@ -244,8 +307,9 @@ struct BwdSched {
       ti.aux = 1 + w / nw;
       ti.kb1 = (T + BK - 1) / BK;
     }
+    ti.kb0 = 0;
     ti.m0 = mb * 2 * BM;
-    ti.n0 = nb * 2 * pair::BN2;
+    ti.n0 = nb * NH * pair::BN2;
     ti.a_row = ti.m0;
     ti.b_row = ti.n0;
     ti.aux2 = 0;
@@ -254,24 +318,30 @@ struct BwdSched {
   __device__ bool producer_wait(const TileInfo&, int, uint64_t, volatile int*, ErrorRecord*) const { return true; }
   __device__ void issue_loads_pair(const TileInfo& ti, int kb, int crank, uint8_t* sA, uint8_t* sB, uint32_t bar) const {
     constexpr uint32_t kBox = 64 * BK * 2;
-    const int m = ti.a_row + crank * BM, n = ti.b_row + crank * BM;
+    const int m = ti.a_row + crank * BM;
     const CUtensorMap* b = &maps->x;
     int k = kb * BK;
     if (ti.aux == 0) {
       const int nk = (I + BK - 1) / BK, z = kb >= nk ? 1 : 0;
       k = (kb - z * nk) * BK;
-      b = z ? &maps->wu : &maps->wg;
+      b = &maps->w[z];
       pair::tma_load_3d_pair(sA, &maps->d_rows, bar, k, m, z);
     } else {
       pair::tma_load_3d_pair(sA, &maps->d_cols, bar, m, k, ti.aux - 1);
       pair::tma_load_3d_pair(sA + kBox, &maps->d_cols, bar, m + 64, k, ti.aux - 1);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      pair::tma_load_2d_pair(sB + j * kBox, b, bar, n + (j >> 1) * pair::BN2 + (j & 1) * 64, k);
+    for (int h = 0; h < NH; ++h) {
+      const int n = ti.b_row + h * pair::BN2 + crank * half_n(ti, h) / 2;
+      pair::tma_load_2d_pair(sB + 2 * h * kBox, b, bar, n, k);
+      pair::tma_load_2d_pair(sB + (2 * h + 1) * kBox, b, bar, n + 64, k);
+    }
   }
-  __device__ uint32_t idesc(const TileInfo& ti) const {
-    return ptx::idesc_f16_f32(2 * BM, pair::BN2, fmt, ti.aux != 0, 1);
+  __device__ int half_n(const TileInfo& ti, int h) const {
+    return max(0, min(pair::BN2, (H - ti.n0 - h * pair::BN2 + 31) / 32 * 32));
+  }
+  __device__ uint32_t idesc(const TileInfo& ti, int n) const {
+    return ptx::idesc_f16_f32(2 * BM, n, fmt, ti.aux != 0, 1);
   }
   __device__ uint64_t a_desc(const TileInfo& ti, uint32_t a, int k) const {
     return ti.aux == 0 ? ptx::sdesc_kmajor_sw128(a + k * 32) : ptx::sdesc_mnmajor_sw128(a + k * 2048, 8192);
@@ -279,31 +349,83 @@ struct BwdSched {
   __device__ uint64_t b_desc(const TileInfo&, uint32_t b, int k) const {
     return ptx::sdesc_mnmajor_sw128(b + k * 2048, 8192);
   }
-  __device__ bool lane_skip(const TileInfo&, int, uint32_t*) const { return false; }
 };
 
 struct BwdEpi : Out16Epi {
-  uint16_t *dx, *dwg, *dwu;
-  long long lddx, lddw;
-  int T, H, I;
-  int vec_x, vec_w;
+  static constexpr bool kRowStores = false;  // gradients have 16-byte aligned rows
+  int T, I;
   const BwdMaps* maps;
   __device__ void begin_tile(const TileInfo& ti, int) {
-    const bool is_x = ti.aux == 0;
-    C = is_x ? dx : ti.aux == 1 ? dwg : dwu;
-    ldc = is_x ? lddx : lddw;
-    M = is_x ? T : I;
-    N = H;
-    vec = is_x ? vec_x : vec_w;
-    tmC = is_x ? &maps->dx : ti.aux == 1 ? &maps->dwg : &maps->dwu;
+    M = ti.aux == 0 ? T : I;
+    tmC = ti.aux == 0 ? &maps->dx : ti.aux == 1 ? &maps->dwg : &maps->dwu;
+  }
+  __device__ bool staged() const { return true; }
+};
+
+template <int NH>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::kThreads, 1)
+    k_gated_bwd(const __grid_constant__ BwdMaps maps, BwdSched<NH> sched, BwdEpi epi, ErrorRecord* err,
+                uint64_t timeout_ns) {
+  sched.maps = &maps;
+  epi.maps = &maps;
+  pair::gemm_core_pair<NH>(&maps.d_rows, &maps.x, sched, epi, err, timeout_ns, -1);
+}
+
+// The same products on the split-K clusters: dx of few rows (over both weights' rows), or small
+// weight gradients over many rows.
+struct DxSplitOp : split::PlainOp {
+  static constexpr int kAccs = 1;
+  uint16_t* dx;
+  long long lddx;
+  int H, I, bn;
+  __device__ int depth() const { return 2 * ((I + BK - 1) / BK); }
+  // k_gate_grad's results, from here on
+  __device__ void prepare(uint8_t*, int, ErrorRecord*) { ptx::griddep_wait(); }
+  __device__ uint32_t idesc(int n) const { return ptx::idesc_f16_f32(split::kRows, n, type, 0, 1); }
+  __device__ uint64_t w_desc(uint32_t w, int k) const { return ptx::sdesc_mnmajor_sw128(w + k * 2048, 8192); }
+  __device__ void loads(int kb, int t0, int n0, uint8_t* x, uint8_t* w, uint64_t* bar) const {
+    const int nk = (I + BK - 1) / BK, z = kb >= nk ? 1 : 0, k = (kb - z * nk) * BK;
+    for (int j = 0; j < bn; j += 64) ptx::tma_load_2d(w + j * BK * 2, tmW + z, bar, n0 + j, k);
+    ptx::tma_load_3d(x, tmX, bar, k, t0, z);
+  }
+  __device__ __forceinline__ void emit(int t, int col, const float (*v)[4]) const {
+    split::store4_16(dx + (size_t)t * lddx, col, H, v[0], type, 1);
+  }
+};
+struct DwSplitOp : split::PlainOp {
+  static constexpr int kAccs = 1;
+  uint16_t *dwg, *dwu;
+  long long lddw;
+  int T, H, bn, mblocks;
+  __device__ int z() const { return (int)blockIdx.y / mblocks; }  // 0 dWg, 1 dWu
+  __device__ int depth() const { return (T + BK - 1) / BK; }
+  __device__ void prepare(uint8_t*, int, ErrorRecord*) { ptx::griddep_wait(); }
+  __device__ uint32_t idesc(int n) const { return ptx::idesc_f16_f32(split::kRows, n, type, 1, 1); }
+  __device__ uint64_t x_desc(uint32_t x, int k) const { return ptx::sdesc_mnmajor_sw128(x + k * 2048, 8192); }
+  __device__ uint64_t w_desc(uint32_t w, int k) const { return ptx::sdesc_mnmajor_sw128(w + k * 2048, 8192); }
+  __device__ void loads(int kb, int t0, int n0, uint8_t* x, uint8_t* w, uint64_t* bar) const {
+    for (int j = 0; j < bn; j += 64) ptx::tma_load_2d(w + j * BK * 2, tmW, bar, n0 + j, kb * BK);
+    ptx::tma_load_3d(x, tmX, bar, t0, kb * BK, z());
+    ptx::tma_load_3d(x + 64 * BK * 2, tmX, bar, t0 + 64, kb * BK, z());
+  }
+  __device__ __forceinline__ void emit(int i, int col, const float (*v)[4]) const {
+    split::store4_16((z() ? dwu : dwg) + (size_t)i * lddw, col, H, v[0], type, 1);
   }
 };
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<2>::kThreads, 1)
-    k_gated_bwd(const __grid_constant__ BwdMaps maps, BwdSched sched, BwdEpi epi, ErrorRecord* err, uint64_t timeout_ns) {
-  sched.maps = &maps;
-  epi.maps = &maps;
-  pair::gemm_core_pair<2>(&maps.d_rows, &maps.x, sched, epi, err, timeout_ns, -1);
+__global__ void __launch_bounds__(split::kThreads, 1)
+    k_gated_dx_split(const __grid_constant__ BwdMaps maps, split::Shape sh, DxSplitOp op, ErrorRecord* err,
+                     uint64_t timeout_ns) {
+  op.tmX = &maps.d_split;
+  op.tmW = maps.w;
+  split::split_core(sh, op, err, timeout_ns);
+}
+__global__ void __launch_bounds__(split::kThreads, 1)
+    k_gated_dw_split(const __grid_constant__ BwdMaps maps, split::Shape sh, DwSplitOp op, ErrorRecord* err,
+                     uint64_t timeout_ns) {
+  op.tmX = &maps.d_cols;
+  op.tmW = &maps.x;
+  split::split_core(sh, op, err, timeout_ns);
 }
 
 namespace {
@@ -314,7 +436,7 @@ CUtensorMap map_128b(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, u
 }
 bool vec16(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * 2 & 15) == 0; }
 CUtensorMap out_map(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, const CUtensorMap& unused) {
-  return vec16(p, (long long)ld) ? make_tmap_2d(p, k16, 2, rows, cols, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE) : unused;
+  return vec16(p, (long long)ld) ? make_tmap_2d(p, k16, 2, rows, cols, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : unused;
 }
 template <class K>
 void allow_smem(K kernel, uint32_t bytes, bool* done) {
@@ -325,6 +447,108 @@ void allow_smem(K kernel, uint32_t bytes, bool* done) {
   if (dev < 64) done[dev] = true;
 }
 constexpr uint32_t kSmemMax = 227 * 1024;
+constexpr int kRingKb = 200;  // the split kernel's ring
+
+template <int NH>
+void launch_gated_pair(const GatedMaps& m, const GatedEpi& e, int T, int I, int H, cudaStream_t stream) {
+  using Cf = pair::PairCfg<NH>;
+  GatedSched<NH> s;
+  s.T = T;
+  s.I = I;
+  s.H = H;
+  s.num_m = (T + 2 * BM - 1) / (2 * BM);
+  s.num_n = (I + s.kCols - 1) / s.kCols;
+  s.group_m = ops::gemm_tuning().pair_group_m;
+  s.fmt = e.fmt;
+  s.maps = nullptr;
+  static bool done[64] = {false};
+  allow_smem(k_gated_pair<NH>, Cf::kSmemBytesSwizzled, done);
+  const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
+  k_gated_pair<NH><<<grid, Cf::kThreads, Cf::kSmemBytesSwizzled, stream>>>(m, s, e, device_error_record(),
+                                                                         default_timeout_ns());
+  GICC_CUDA(cudaGetLastError());
+}
+
+template <int NH>
+void launch_gated_bwd(const BwdMaps& m, int T, int H, int I, bool need_x, bool need_w, int fmt, unsigned int* counter,
+                      cudaStream_t stream) {
+  using Cf = pair::PairCfg<NH>;
+  BwdSched<NH> s;
+  s.counter = counter;
+  s.T = T;
+  s.H = H;
+  s.I = I;
+  s.mx = (T + 2 * BM - 1) / (2 * BM);
+  s.mw = (I + 2 * BM - 1) / (2 * BM);
+  s.nn = (H + NH * pair::BN2 - 1) / (NH * pair::BN2);
+  s.nx = need_x ? s.mx * s.nn : 0;
+  s.nw = need_w ? s.mw * s.nn : 0;
+  s.x_first = 2LL * I >= T;
+  s.group_m = ops::gemm_tuning().pair_group_m;
+  s.fmt = fmt;
+  s.maps = nullptr;
+  BwdEpi e;
+  e.fmt = fmt;
+  e.N = H;
+  e.T = T;
+  e.I = I;
+  e.vec = 1;
+  e.maps = nullptr;
+  static bool done[64] = {false};
+  allow_smem(k_gated_bwd<NH>, Cf::kSmemBytesSwizzled, done);
+  const int grid = 2 * std::min(s.num_tiles(), num_sms() / 2);
+  split::launch_dependent(k_gated_bwd<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
+                          device_error_record(), default_timeout_ns());
+}
+
+// Where the backward products run: dx and the weight gradients each on CTA pairs (together, in
+// one launch) or on the split-K clusters, by expected time.
+struct BwdPlan {
+  bool x_split = false, w_split = false;
+  int nh = 2;
+  split::Plan px, pw;
+};
+BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
+  const int pairs = num_sms() / 2;
+  const int kx = 2 * ((I + BK - 1) / BK), kw = (T + BK - 1) / BK;
+  BwdPlan best;
+  if (need_x && (tile == 0 || tile == 1))
+    best.px = split::plan(T, H, 2 * I, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dx_split), 64, 1, kx);
+  if (need_w && (tile == 0 || tile == 1))
+    best.pw = split::plan(I, H, T, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dw_split), 64, 2, kw,
+                          true);
+  if (tile) {
+    best.x_split = tile == 1 && need_x;
+    best.w_split = tile == 1 && need_w;
+    best.nh = tile == 3 ? 1 : 2;
+    return best;
+  }
+  // us of the pairs' launch: a tile's k-blocks and what its epilogue costs beside them, shared by
+  // the pairs; at the end the last tiles, or the deepest alone
+  auto pair_us = [&](int nh, bool x, bool w) {
+    if (!x && !w) return 0.0;
+    const double nn = std::ceil((double)H / (nh * pair::BN2));
+    const double nx = x ? std::ceil(T / 256.0) * nn : 0, nw = w ? 2 * std::ceil(I / 256.0) * nn : 0;
+    const double busy = std::min(1.0, (nx + nw) / pairs), step = nh == 2 ? 0.60 + 0.14 * busy : 0.33 + 0.07 * busy;
+    const double cx = step * kx + 2.5 * nh, cw = step * kw + 2.5 * nh;
+    const double longest = std::max(nx ? cx : 0.0, nw ? cw : 0.0), last = nx && nw ? std::min(cx, cw) : longest;
+    const double even = nx + nw <= pairs ? longest : (nx * cx + nw * cw) / pairs + 0.5 * last;
+    return std::max(even, longest) + 8.0;
+  };
+  double cost = -1;
+  for (int nh = 2; nh >= 1; --nh)
+    for (int xs = 0; xs <= (need_x ? 1 : 0); ++xs)
+      for (int ws = 0; ws <= (need_w ? 1 : 0); ++ws) {
+        const double c = pair_us(nh, need_x && !xs, need_w && !ws) + (xs ? best.px.us + 2 : 0) + (ws ? best.pw.us + 2 : 0);
+        if (cost < 0 || c < cost) {
+          cost = c;
+          best.x_split = xs;
+          best.w_split = ws;
+          best.nh = nh;
+        }
+      }
+  return best;
+}
 
 void check_16(const char* who, int fmt, int kind) {
   if (fmt < 0 || fmt > 1) throw std::runtime_error(std::string(who) + ": fmt must be 0 (f16) or 1 (bf16)");
@@ -340,8 +564,11 @@ void check_rows(const char* who, const char* name, const void* p, long long ld, 
 
 namespace ops {
 
+// dg and du, rows of 128-byte multiples; then the tile counter
+static int grad_pitch(int I) { return (I + 63) / 64 * 64; }
+static size_t grad_counter_at(int T, int I) { return (size_t)2 * T * grad_pitch(I) * 2; }
 size_t gated_saved_floats(int T, int I) { return 2 * ffn::saved_plane(T, I); }
-int gated_grad_pitch(int I) { return (I + 63) / 64 * 64; }
+size_t gated_grad_bytes(int T, int I) { return grad_counter_at(T, I) + 16; }
 
 void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I, long long ldx,
                   long long ldg, long long ldu, long long ldh, int kind, int fmt, float* saved, int tile,
@@ -356,17 +583,21 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   check_rows(who, "w_gate", w_gate, ldg, H);
   check_rows(who, "w_up", w_up, ldu, H);
   if (h == nullptr || ldh < I) throw std::runtime_error("gicc::gated_linear: h needs rows of at least I elements");
-  if (tile < 0 || tile > 2) throw std::runtime_error("gicc::gated_linear: tile must be 0 (by shape), 1 (split) or 2 (pairs)");
-  if (tile == 0) tile = T <= 256 ? 1 : 2;
+  if (tile < 0 || tile > 3)
+    throw std::runtime_error("gicc::gated_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
+  if (tile == 0) tile = split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
   if (tile == 1) {
-    const split::Plan p = split::plan(T, I, H, 2, 0);
+    const split::Plan p = split::plan(T, I, H, 2, kRingKb, 0, reinterpret_cast<const void*>(k_gated_split));
     GatedSplitOp op;
     op.h = static_cast<uint16_t*>(h);
     op.ldh = ldh;
     op.T = T;
+    op.H = H;
     op.I = I;
     op.kind = kind;
     op.type = fmt;
+    op.bn = p.sh.bn;
+    op.tmX = op.tmW = op.tmU = nullptr;
     op.vec = (reinterpret_cast<uintptr_t>(h) & 7) == 0 && ldh % 4 == 0;
     op.saved = saved;
     static bool done[64] = {false};
@@ -376,21 +607,11 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
                            map_128b(w_up, I, H, ldu, p.sh.bn), p.sh, op, device_error_record(), default_timeout_ns());
     return;
   }
-  using Cf = pair::PairCfg<2>;
   GatedMaps m;
   m.x = map_128b(x, T, H, ldx, BM);
   m.g = map_128b(w_gate, I, H, ldg, BM);
   m.u = map_128b(w_up, I, H, ldu, BM);
   m.h = out_map(h, T, I, ldh, m.x);
-  GatedSched s;
-  s.T = T;
-  s.I = I;
-  s.H = H;
-  s.num_m = (T + 2 * BM - 1) / (2 * BM);
-  s.num_n = (I + pair::BN2 - 1) / pair::BN2;
-  s.group_m = gemm_tuning().pair_group_m;
-  s.fmt = fmt;
-  s.maps = nullptr;
   GatedEpi e;
   e.C = static_cast<uint16_t*>(h);
   e.ldc = ldh;
@@ -400,17 +621,14 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   e.vec = vec16(h, ldh);
   e.kind = kind;
   e.saved = saved;
-  static bool done[64] = {false};
-  allow_smem(k_gated_pair, Cf::kSmemBytesStaged, done);
-  const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
-  k_gated_pair<<<grid, Cf::kThreads, Cf::kSmemBytesStaged, stream>>>(m, s, e, device_error_record(), default_timeout_ns());
-  GICC_CUDA(cudaGetLastError());
+  if (tile == 2) launch_gated_pair<2>(m, e, T, I, H, stream);
+  else launch_gated_pair<1>(m, e, T, I, H, stream);
 }
 
 void gated_linear_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* saved,
                            void* work, void* dx, void* dw_gate, void* dw_up, int T, int H, int I, long long lddh,
                            long long ldx, long long ldg, long long ldu, long long lddx, long long lddw, int kind, int fmt,
-                           cudaStream_t stream) {
+                           int tile, cudaStream_t stream) {
   NvtxRange nvtx("gicc::ops::gated_linear_backward");
   using namespace ffn;
   const char* who = "gicc::gated_linear_backward";
@@ -424,59 +642,70 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     throw std::runtime_error("gicc::gated_linear_backward: dh, saved and a 16-byte aligned work area are needed");
   if ((dw_gate == nullptr) != (dw_up == nullptr))
     throw std::runtime_error("gicc::gated_linear_backward: both weight gradients or none");
-  if ((dx != nullptr && lddx < H) || (dw_gate != nullptr && lddw < H))
-    throw std::runtime_error("gicc::gated_linear_backward: gradients need rows of at least H elements");
+  if (tile < 0 || tile > 3)
+    throw std::runtime_error("gicc::gated_linear_backward: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   if (dx == nullptr && dw_gate == nullptr) return;
-  const int Ip = gated_grad_pitch(I);
+  if (dx != nullptr) check_rows(who, "dx", dx, lddx, H);
+  if (dw_gate != nullptr) {
+    check_rows(who, "dw_gate", dw_gate, lddw, H);
+    check_rows(who, "dw_up", dw_up, lddw, H);
+  }
+  const int Ip = grad_pitch(I);
+  const BwdPlan plan = plan_bwd(T, H, I, dx != nullptr, dw_gate != nullptr, tile);
   uint16_t* dgu = static_cast<uint16_t*>(work);
-  const long long blocks = (long long)((T + 31) / 32) * (saved_cols(I) / 16);
-  const int ggrid = (int)std::min<long long>((blocks + 7) / 8, (long long)num_sms() * 8);
+  unsigned int* counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(work) + grad_counter_at(T, I));
+  const dim3 ggrid((saved_cols(I) + kGradCols - 1) / kGradCols, std::min((T + 31) / 32, 32768));
   k_gate_grad<<<ggrid, 256, 0, stream>>>(static_cast<const uint16_t*>(dh), lddh, saved, dgu, T, I, Ip, kind, fmt,
-                                         vec16(dh, lddh) ? 1 : 0);
+                                         vec16(dh, lddh) ? 1 : 0, counter, (unsigned)(num_sms() / 2));
   GICC_CUDA(cudaGetLastError());
 
-  using Cf = pair::PairCfg<2>;
   BwdMaps m;
   m.d_rows = make_tmap_3d(dgu, k16, 2, 2, T, I, Ip, (uint64_t)T * Ip, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   m.d_cols = make_tmap_3d(dgu, k16, 2, 2, T, I, Ip, (uint64_t)T * Ip, 64, BK, CU_TENSOR_MAP_SWIZZLE_128B);
-  m.wg = map_128b(w_gate, I, H, ldg, 64);
-  m.wu = map_128b(w_up, I, H, ldu, 64);
+  m.w[0] = map_128b(w_gate, I, H, ldg, 64);
+  m.w[1] = map_128b(w_up, I, H, ldu, 64);
   m.x = map_128b(x, T, H, ldx, 64);
   m.dx = dx ? out_map(dx, T, H, lddx, m.x) : m.x;
   m.dwg = dw_gate ? out_map(dw_gate, I, H, lddw, m.x) : m.x;
   m.dwu = dw_up ? out_map(dw_up, I, H, lddw, m.x) : m.x;
-  BwdSched s;
-  s.T = T;
-  s.H = H;
-  s.I = I;
-  s.mx = (T + 2 * BM - 1) / (2 * BM);
-  s.mw = (I + 2 * BM - 1) / (2 * BM);
-  s.nn = (H + Cf::kCols - 1) / Cf::kCols;
-  s.nx = dx ? s.mx * s.nn : 0;
-  s.nw = dw_gate ? s.mw * s.nn : 0;
-  s.x_first = 2LL * I >= T;
-  s.group_m = gemm_tuning().pair_group_m;
-  s.fmt = fmt;
-  s.maps = nullptr;
-  BwdEpi e;
-  e.fmt = fmt;
-  e.dx = static_cast<uint16_t*>(dx);
-  e.dwg = static_cast<uint16_t*>(dw_gate);
-  e.dwu = static_cast<uint16_t*>(dw_up);
-  e.lddx = lddx;
-  e.lddw = lddw;
-  e.T = T;
-  e.H = H;
-  e.I = I;
-  e.vec_x = dx && vec16(dx, lddx);
-  e.vec_w = dw_gate && vec16(dw_gate, lddw) && vec16(dw_up, lddw);
-  e.maps = nullptr;
-  static bool done[64] = {false};
-  allow_smem(k_gated_bwd, Cf::kSmemBytesStaged, done);
-  const int tiles = s.nx + 2 * s.nw;
-  const int grid = 2 * std::min(tiles, num_sms() / 2);
-  k_gated_bwd<<<grid, Cf::kThreads, Cf::kSmemBytesStaged, stream>>>(m, s, e, device_error_record(), default_timeout_ns());
-  GICC_CUDA(cudaGetLastError());
+  m.d_split = plan.x_split ? make_tmap_3d(dgu, k16, 2, 2, T, I, Ip, (uint64_t)T * Ip, plan.px.sh.xrows, BK,
+                                          CU_TENSOR_MAP_SWIZZLE_128B)
+                           : m.d_rows;
+  const bool pair_x = dx != nullptr && !plan.x_split, pair_w = dw_gate != nullptr && !plan.w_split;
+  if (pair_x || pair_w) {
+    if (plan.nh == 2) launch_gated_bwd<2>(m, T, H, I, pair_x, pair_w, fmt, counter, stream);
+    else launch_gated_bwd<1>(m, T, H, I, pair_x, pair_w, fmt, counter, stream);
+  }
+  if (plan.x_split) {
+    DxSplitOp op;
+    op.type = fmt;
+    op.tmX = op.tmW = nullptr;
+    op.dx = static_cast<uint16_t*>(dx);
+    op.lddx = lddx;
+    op.H = H;
+    op.I = I;
+    op.bn = plan.px.sh.bn;
+    static bool done[64] = {false};
+    allow_smem(k_gated_dx_split, kSmemMax, done);
+    split::launch_clusters(k_gated_dx_split, plan.px.grid, plan.px.splits, split::kThreads, plan.px.smem, true, stream, m,
+                           plan.px.sh, op, device_error_record(), default_timeout_ns());
+  }
+  if (plan.w_split) {
+    DwSplitOp op;
+    op.type = fmt;
+    op.tmX = op.tmW = nullptr;
+    op.dwg = static_cast<uint16_t*>(dw_gate);
+    op.dwu = static_cast<uint16_t*>(dw_up);
+    op.lddw = lddw;
+    op.T = T;
+    op.H = H;
+    op.bn = plan.pw.sh.bn;
+    op.mblocks = plan.pw.sh.mblocks;
+    static bool done[64] = {false};
+    allow_smem(k_gated_dw_split, kSmemMax, done);
+    split::launch_clusters(k_gated_dw_split, plan.pw.grid, plan.pw.splits, split::kThreads, plan.pw.smem, true, stream, m,
+                           plan.pw.sh, op, device_error_record(), default_timeout_ns());
+  }
 }
 
 }  // namespace ops

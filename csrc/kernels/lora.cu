@@ -45,14 +45,18 @@ struct TileLists {
 
 // ---- v = s A x ---------------------------------------------------------------------------------
 // Grid (S, G, ceil(T / 128)): a cluster of S CTAs splits K for one 128-row tile and the adapters
-// i with i % G == blockIdx.y of the tile's list (one group when there are many tiles).  Bound by
-// reading x and the used A[a] once; the MMAs (128 x r per k-block) are small beside that.
+// i with i % G == blockIdx.y of the tile's list (one group when there are many tiles).  The
+// group's adapters go through the MMA side by side, `cap` at a time (128 columns: one MMA per
+// k-step for all of them, and x is loaded once for all), into two TMEM accumulators in turn; a
+// TMEM reader thread owns a row and keeps the columns of that row's adapter in registers.
+// Bound by reading x and the used A[a]; the MMAs are small beside that.
 struct DownArgs {
   const int* adapter;
   const float* scale;
   uint16_t* v;
   int T, K, L, r;
-  int rp;      // r rounded up to 16: columns of the MMA
+  int rp;      // r rounded up to 16: columns of one adapter
+  int cap;     // adapters side by side
   int xrows;   // rows of an x box
   int groups;
   int stages;
@@ -60,16 +64,22 @@ struct DownArgs {
   TileLists lists;  // count null: not wanted
 };
 
-// With its lists this leaves room for a k_lora_split CTA on the same SM.
-constexpr uint32_t kDownRing = 80 * 1024;
-__host__ __device__ constexpr uint32_t down_stage(int rp) { return split::kXBytes + rp * BK * 2; }
-__host__ __device__ constexpr uint32_t down_ring(int rp, int stages) {
-  const uint32_t ring = stages * down_stage(rp), part = split::kRows * split::pitch(1, rp) * 4;
+constexpr int kDownCols = 128;  // columns of an accumulator
+// Beside a k_lora_split CTA's ring both fit an SM.
+constexpr uint32_t kDownRing = 92 * 1024;
+__host__ __device__ constexpr uint32_t down_stage(int xrows, int cols) { return split::x_bytes(xrows) + cols * BK * 2; }
+// as split::ring_bytes: the MMA reads 128 rows from the last x box on
+__host__ __device__ constexpr uint32_t down_ring(int rp, int cols, int xrows, int stages) {
+  uint32_t ring = stages * down_stage(xrows, cols);
+  const uint32_t reach = (stages - 1) * split::x_bytes(xrows) + split::kRows * BK * 2;
+  const uint32_t part = split::kRows * split::pitch(1, rp) * 4;
+  if (reach > ring) ring = reach;
   return ((ring > part ? ring : part) + 127) / 128 * 128;
 }
+constexpr uint32_t kDownBar = (2 * split::kMaxStages + 5) * 8 + 8;
 struct DownLists {
-  LaneLists<split::kRows> tile;
-  LaneLists<kPairRows> pair;  // shared memory only where the pair lists are wanted
+  LaneLists<split::kRows, false> tile;
+  alignas(16) LaneLists<kPairRows> pair;  // shared memory only where the pair lists are wanted
 };
 
 __global__ void __launch_bounds__(split::kThreads)
@@ -77,18 +87,19 @@ __global__ void __launch_bounds__(split::kThreads)
                 ErrorRecord* err, uint64_t timeout_ns) {
   extern __shared__ uint8_t down_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(down_smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = p.stages;
-  const uint32_t abytes = p.rp * BK * 2;
+  const int stages = p.stages, cap = p.cap;
+  const uint32_t xb = split::x_bytes(p.xrows), ab = p.rp * BK * 2;  // one x box, one adapter's box
   uint8_t* sX = smem;
-  uint8_t* sA = smem + stages * split::kXBytes;
-  uint8_t* after = smem + down_ring(p.rp, stages);
+  uint8_t* sA = smem + stages * xb;
+  uint8_t* after = smem + down_ring(p.rp, cap * p.rp, p.xrows, stages);
   uint64_t* full = reinterpret_cast<uint64_t*>(after);
   uint64_t* empty = full + split::kMaxStages;
   uint64_t* tfull = empty + split::kMaxStages;
-  uint64_t* drain = tfull + 1;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  DownLists& lists = *reinterpret_cast<DownLists*>(after + split::kBarBytes);
+  DownLists& lists = *reinterpret_cast<DownLists*>(after + (kDownBar + 15) / 16 * 16);
   float* part = reinterpret_cast<float*>(smem);
 
   const uint32_t warp = ptx::warp_id();
@@ -98,14 +109,16 @@ __global__ void __launch_bounds__(split::kThreads)
   const int g = blockIdx.y;
   const int t0 = (int)blockIdx.z * split::kRows;
   const int rows = min(split::kRows, p.T - t0);
-  const uint32_t ncols = split::tmem_cols(p.rp);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&empty[s], 1);
     }
-    ptx::mbar_init(tfull, 1);
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(&tfull[a], 1);
+      ptx::mbar_init(&tempty[a], 4);
+    }
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -113,7 +126,7 @@ __global__ void __launch_bounds__(split::kThreads)
     ptx::prefetch_tmap(&tmA);
   }
   if (warp == 1) {
-    ptx::tmem_alloc(tmem_slot, ncols);
+    ptx::tmem_alloc(tmem_slot, 2 * kDownCols);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
@@ -124,7 +137,136 @@ __global__ void __launch_bounds__(split::kThreads)
   const uint32_t tmem = *tmem_slot;
   // One CTA per tile reports indexes out of range.
   lists.tile.build(p.adapter, t0, p.T, p.L, g == 0 && c == 0 ? err : nullptr);
+  const int nkb = (p.K + BK - 1) / BK;
+  const int kb0 = (int)((long long)nkb * c / S), nk = (int)((long long)nkb * (c + 1) / S) - kb0;
   const int n = lists.tile.n;
+  const int mine = n > g ? (n - g + p.groups - 1) / p.groups : 0;  // adapters of this group
+  const int passes = (mine + cap - 1) / cap;  // 0: no row of this tile is this cluster's
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      for (int ps = 0; ps < passes && !*abort_flag; ++ps) {
+        const int na = min(cap, mine - ps * cap);
+        for (int k = 0; k < nk; ++k) {
+          if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
+            if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
+            *abort_flag = 1;
+            break;
+          }
+          ptx::mbar_arrive_expect_tx(&full[stage], xb + na * ab);
+          ptx::tma_load_2d(sX + stage * xb, &tmX, &full[stage], (kb0 + k) * BK, t0);
+          for (int j = 0; j < na; ++j)
+            ptx::tma_load_3d(sA + (stage * cap + j) * ab, &tmA, &full[stage], (kb0 + k) * BK, 0,
+                             lists.tile.list[g + (ps * cap + j) * p.groups]);
+          ++issued;
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (*abort_flag) {
+        for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+          ptx::mbar_wait(&full[i % stages], (i / stages) & 1, 20000000ull, nullptr);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool issued = false;
+      for (int ps = 0; ps < passes && !*abort_flag; ++ps) {
+        const int acc = ps & 1, na = min(cap, mine - ps * cap);
+        const uint32_t idesc = ptx::idesc_f16_f32(split::kRows, na * p.rp, p.fmt, 0, 0);
+        bool ok = ptx::mbar_wait(&tempty[acc], ((ps >> 1) & 1) ^ 1, timeout_ns, abort_flag);
+        for (int k = 0; ok && k < nk; ++k) {
+          ok = ptx::mbar_wait(&full[stage], phase, timeout_ns, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          const uint32_t x = ptx::smem_u32(sX + stage * xb), a = ptx::smem_u32(sA + stage * cap * ab);
+#pragma unroll
+          for (int q = 0; q < BK / 16; ++q)
+            ptx::mma_f16_ss(tmem + acc * kDownCols, ptx::sdesc_kmajor_sw128(x + q * 32),
+                            ptx::sdesc_kmajor_sw128(a + q * 32), idesc, (k > 0 || q > 0) ? 1u : 0u);
+          issued = true;
+          ptx::mma_commit(&empty[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) {
+          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 2, 0);
+          *abort_flag = 1;
+          break;
+        }
+        ptx::mma_commit(&tfull[acc]);
+      }
+      if (*abort_flag && issued) {
+        ptx::mma_commit(drain);
+        ptx::mbar_wait(drain, 0, 20000000ull, nullptr);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const int row = q * 32 + (int)lane;
+    // this row's adapter: which pass computes it, and where among the pass's columns
+    int my = -1;
+    if (row < rows) {
+      const int a = p.adapter[t0 + row];
+      if (a >= 0 && a < p.L) {
+        const int s = lists.tile.slot(a);
+        if (s % p.groups == g) my = s / p.groups;
+      }
+    }
+    float v[kMaxRank];
+#pragma unroll
+    for (int i = 0; i < kMaxRank; ++i) v[i] = 0.f;
+    for (int ps = 0; ps < passes; ++ps) {
+      const int acc = ps & 1, na = min(cap, mine - ps * cap);
+      if (!ptx::mbar_wait_long(&tfull[acc], (ps >> 1) & 1, timeout_ns, abort_flag)) {
+        if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 3, 0);
+        *abort_flag = 1;
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * kDownCols;
+      for (int j = 0; j < na; ++j) {
+        const bool is_mine = my == ps * cap + j;
+        if (!__any_sync(0xffffffffu, is_mine)) continue;
+#pragma unroll
+        for (int ch = 0; ch < kMaxRank / 16; ++ch) {
+          if (ch * 16 >= p.rp) break;
+          uint32_t r[16];
+          ptx::tmem_ld16(tbase + j * p.rp + ch * 16, r);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (is_mine) v[ch * 16 + i] = __uint_as_float(r[i]);
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&tempty[acc]);
+    }
+    // Every MMA has read its operands (the last pass's barrier), so the ring takes the partial.
+    if (my >= 0 && !*abort_flag) {
+      float* dst = part + row * split::pitch(1, p.rp);
+#pragma unroll
+      for (int ch = 0; ch < kMaxRank / 4; ++ch) {
+        if (ch * 4 >= p.rp) break;
+        *reinterpret_cast<float4*>(dst + ch * 4) = make_float4(v[ch * 4], v[ch * 4 + 1], v[ch * 4 + 2], v[ch * 4 + 3]);
+      }
+    }
+    __syncwarp();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
   if (p.lists.count != nullptr && g == 0 && c == 0 && (blockIdx.z & 1) == 0) {
     // the list of the 256-row tile that starts here, for the CTA-pair projection
     const int tile = blockIdx.z >> 1;
@@ -135,108 +277,16 @@ __global__ void __launch_bounds__(split::kThreads)
       p.lists.skip[(size_t)tile * p.lists.cap * 8 + i] = lists.pair.skip[0][i];
     if (threadIdx.x == 0) p.lists.count[tile] = m;
   }
-  const int nkb = (p.K + BK - 1) / BK;
-  const int kb0 = (int)((long long)nkb * c / S), nk = (int)((long long)nkb * (c + 1) / S) - kb0;
-  const int mine = n > g ? (n - g + p.groups - 1) / p.groups : 0;
-  const int steps = mine * nk;  // adapter-major; 0: no row of this tile is this cluster's
-
-  if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t tx = p.xrows * BK * 2 + abytes;
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      for (int i = 0; i < steps; ++i) {
-        if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
-          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
-          *abort_flag = 1;
-          break;
-        }
-        const int j = i / nk, kx = (kb0 + i - j * nk) * BK;
-        ptx::mbar_arrive_expect_tx(&full[stage], tx);
-        ptx::tma_load_2d(sX + stage * split::kXBytes, &tmX, &full[stage], kx, t0);
-        ptx::tma_load_3d(sA + stage * abytes, &tmA, &full[stage], kx, 0, lists.tile.list[g + j * p.groups]);
-        issued = i + 1;
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-      if (*abort_flag) {
-        for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-          ptx::mbar_wait(&full[i % stages], (i / stages) & 1, 20000000ull, nullptr);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0 && steps > 0) {
-      const uint32_t idesc = ptx::idesc_f16_f32(split::kRows, p.rp, p.fmt, 0, 0);
-      int stage = 0;
-      uint32_t phase = 0;
-      int i = 0;
-      for (; i < steps; ++i) {
-        if (!ptx::mbar_wait(&full[stage], phase, timeout_ns, abort_flag)) {
-          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 2, 0);
-          *abort_flag = 1;
-          break;
-        }
-        ptx::tc_fence_after();
-        const int j = i / nk;
-        const uint32_t* skip = lists.tile.skip[g + j * p.groups];
-        const uint32_t x = ptx::smem_u32(sX + stage * split::kXBytes), a = ptx::smem_u32(sA + stage * abytes);
-#pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          ptx::mma_f16_ss_lanes(tmem, ptx::sdesc_kmajor_sw128(x + k * 32), ptx::sdesc_kmajor_sw128(a + k * 32), idesc,
-                                (i - j * nk > 0 || k > 0) ? 1u : 0u, skip);
-        ptx::mma_commit(&empty[stage]);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-      if (i == steps) {
-        ptx::mma_commit(tfull);
-      } else if (i > 0) {
-        ptx::mma_commit(drain);
-        ptx::mbar_wait(drain, 0, 20000000ull, nullptr);
-      }
-    }
-    __syncwarp();
-  } else if (steps > 0) {
-    const int q = warp & 3;
-    const int row = q * 32 + (int)lane;
-    if (!ptx::mbar_wait_long(tfull, 0, timeout_ns, abort_flag)) {
-      if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 3, 0);
-      *abort_flag = 1;
-    } else if (q * 32 < rows) {
-      ptx::tc_fence_after();
-      const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16);
-      float* dst = part + row * split::pitch(1, p.rp);
-      for (int col = 0; col < p.rp; col += 16) {
-        uint32_t r[16];
-        ptx::tmem_ld16(tbase + col, r);
-        ptx::tmem_ld_wait();
-        if (row < rows) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(dst + col + 4 * j) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-        }
-      }
-    }
-    __syncwarp();
-  }
-  ptx::tc_fence_before();
-  __syncthreads();
   pair::cluster_sync();
-  if (steps > 0 && !*abort_flag) {
+  if (passes > 0 && !*abort_flag) {
     const int g4 = p.r / 4;
     const int items = rows * g4;
     const uint32_t base = ptx::smem_u32(part);
     const int j1 = (int)((long long)items * (c + 1) / S);
     for (int j = (int)((long long)items * c / S) + (int)threadIdx.x; j < j1; j += split::kThreads) {
       const int row = j / g4, col = (j - row * g4) * 4;
-      const int a = LaneLists<split::kRows>::at(p.adapter, t0 + row, p.T, p.L);
-      if (a < 0 || lists.tile.slot(a) % p.groups != g) continue;
+      const int a = p.adapter[t0 + row];
+      if (a < 0 || a >= p.L || lists.tile.slot(a) % p.groups != g) continue;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       const uint32_t off = base + (row * split::pitch(1, p.rp) + col) * 4;
       for (int s = 0; s < S; ++s) {
@@ -254,22 +304,22 @@ __global__ void __launch_bounds__(split::kThreads)
   pair::cluster_sync();
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, ncols);
+    ptx::tmem_dealloc(tmem, 2 * kDownCols);
   }
 }
 
 // ---- the projection for few rows ---------------------------------------------------------------
-struct LoraSplitOp {
+struct LoraSplitOp : split::PlainOp {
   static constexpr int kAccs = 1;
   const int* adapter;
   uint16_t* y;
   long long ldy;
-  int T, N, L, r, rc;  // rc: k-blocks of 64 per adapter
-  int type, vec, bn;
+  int T, N, K, L, r, rc;  // rc: k-blocks of 64 per adapter
+  int vec;
   const CUtensorMap* tmV;  // set by the kernel
   const CUtensorMap* tmB;
   const LaneLists<split::kRows>* lists;
-  __device__ int fmt() const { return type; }
+  __device__ int depth() const { return (K + BK - 1) / BK; }
   __device__ void prepare(uint8_t* smem, int t0, ErrorRecord*) {
     auto* l = reinterpret_cast<LaneLists<split::kRows>*>(smem);
     l->build(adapter, t0, T, L, nullptr);  // k_lora_down reports indexes out of range
@@ -281,7 +331,7 @@ struct LoraSplitOp {
     e1 = n * (c + 1) / S;
   }
   __device__ void extra_wait() const { ptx::griddep_wait(); }
-  __device__ void extra_loads(int e, int t0, int n0, void* sX, void* sW, uint64_t* bar) const {
+  __device__ void extra_loads(int e, int t0, int n0, uint8_t* sX, uint8_t* sW, uint64_t* bar) const {
     const int s = e / rc, k = (e - s * rc) * BK;
     ptx::tma_load_2d(sX, tmV, bar, k, t0);
     ptx::tma_load_3d(sW, tmB, bar, k, n0, lists->list[s]);
@@ -289,8 +339,7 @@ struct LoraSplitOp {
   __device__ void extra_mma(int e, uint32_t d, uint32_t x, uint32_t w, uint32_t idesc) const {
     const int s = e / rc, left = r - (e - s * rc) * BK;
     for (int k = 0; k < BK / 16 && k * 16 < left; ++k)
-      ptx::mma_f16_ss_lanes(d, ptx::sdesc_kmajor_sw128(x + k * 32), ptx::sdesc_kmajor_sw128(w + k * 32), idesc, 1u,
-                            lists->skip[s]);
+      ptx::mma_f16_ss_lanes(d, x_desc(x, k), w_desc(w, k), idesc, 1u, lists->skip[s]);
   }
   __device__ __forceinline__ void emit(int t, int col, const float (*v)[4]) const {
     split::store4_16(y + (size_t)t * ldy, col, N, v[0], type, vec);
@@ -303,9 +352,11 @@ __global__ void __launch_bounds__(split::kThreads, 1)
     k_lora_split(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmB, split::Shape sh,
                  LoraSplitOp op, ErrorRecord* err, uint64_t timeout_ns) {
+  op.tmX = &tmX;
+  op.tmW = &tmW;
   op.tmV = &tmV;
   op.tmB = &tmB;
-  split::split_core(&tmX, &tmW, &tmW, sh, op, err, timeout_ns);
+  split::split_core(sh, op, err, timeout_ns);
 }
 
 // ---- the projection on CTA pairs ---------------------------------------------------------------
@@ -313,9 +364,12 @@ struct LoraMaps {
   CUtensorMap x, w, v, b, y;
 };
 
+template <int NH>
 struct LoraSched {
   static constexpr int kCommWarps = 0;
   static constexpr bool kOwnOperands = true;
+  static constexpr bool kLanes = true;
+  static constexpr bool kDependent = true;
   int T, N, K, rc;
   int num_m, num_n, group_m;
   int fmt;
@@ -328,39 +382,43 @@ struct LoraSched {
     raster(t, num_m, num_n, group_m, mb, nb);
     TileInfo ti;
     ti.m0 = mb * kPairRows;
-    ti.n0 = nb * 2 * pair::BN2;
+    ti.n0 = nb * NH * pair::BN2;
     ti.a_row = ti.m0;
     ti.b_row = ti.n0;
     ti.kb0 = 0;
-    ti.kb1 = weight_blocks() + __ldg(lists.count + mb) * rc;
+    ti.kb1 = weight_blocks() + (int)ptx::ld_cg(lists.count + mb) * rc;
     ti.aux = mb * lists.cap;
     ti.aux2 = 0;
     return ti;
   }
   __device__ bool producer_wait(const TileInfo&, int, uint64_t, volatile int*, ErrorRecord*) const { return true; }
   __device__ void issue_loads_pair(const TileInfo& ti, int kb, int crank, uint8_t* sA, uint8_t* sB, uint32_t bar) const {
-    const int m = ti.a_row + crank * BM, n = ti.b_row + crank * BM;
+    const int m = ti.a_row + crank * BM;
+    const int n = ti.b_row + crank * half_n(ti, 0) / 2, n1 = ti.b_row + pair::BN2 + crank * half_n(ti, 1) / 2;
     const int e = kb - weight_blocks();
     if (e < 0) {
       pair::tma_load_2d_pair(sA, &maps->x, bar, kb * BK, m);
       pair::tma_load_2d_pair(sB, &maps->w, bar, kb * BK, n);
-      pair::tma_load_2d_pair(sB + pair::kBBytes, &maps->w, bar, kb * BK, n + pair::BN2);
+      if constexpr (NH == 2) pair::tma_load_2d_pair(sB + pair::kBBytes, &maps->w, bar, kb * BK, n1);
     } else {
       const int s = e / rc, k = (e - s * rc) * BK;
-      const int a = __ldg(lists.list + ti.aux + s);
+      const int a = (int)ptx::ld_cg(lists.list + ti.aux + s);
       pair::tma_load_2d_pair(sA, &maps->v, bar, k, m);
       pair::tma_load_3d_pair(sB, &maps->b, bar, k, n, a);
-      pair::tma_load_3d_pair(sB + pair::kBBytes, &maps->b, bar, k, n + pair::BN2, a);
+      if constexpr (NH == 2) pair::tma_load_3d_pair(sB + pair::kBBytes, &maps->b, bar, k, n1, a);
     }
   }
-  __device__ uint32_t idesc(const TileInfo&) const { return ptx::idesc_f16_f32(2 * BM, pair::BN2, fmt, 0, 0); }
+  __device__ int half_n(const TileInfo& ti, int h) const {
+    return max(0, min(pair::BN2, (N - ti.n0 - h * pair::BN2 + 31) / 32 * 32));
+  }
+  __device__ uint32_t idesc(const TileInfo&, int n) const { return ptx::idesc_f16_f32(2 * BM, n, fmt, 0, 0); }
   __device__ uint64_t a_desc(const TileInfo&, uint32_t a, int k) const { return ptx::sdesc_kmajor_sw128(a + k * 32); }
   __device__ uint64_t b_desc(const TileInfo&, uint32_t b, int k) const { return ptx::sdesc_kmajor_sw128(b + k * 32); }
   __device__ bool lane_skip(const TileInfo& ti, int kb, uint32_t* skip) const {
     const int e = kb - weight_blocks();
     if (e < 0) return false;
     const uint4* p = reinterpret_cast<const uint4*>(lists.skip + (size_t)(ti.aux + e / rc) * 8);
-    const uint4 a = __ldg(p), b = __ldg(p + 1);
+    const uint4 a = ptx::ld_v4_cg(p), b = ptx::ld_v4_cg(p + 1);
     skip[0] = a.x;
     skip[1] = a.y;
     skip[2] = a.z;
@@ -373,12 +431,13 @@ struct LoraSched {
   }
 };
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<2>::kThreads, 1)
-    k_lora_pair(const __grid_constant__ LoraMaps maps, LoraSched sched, Out16Epi epi, ErrorRecord* err,
+template <int NH>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::kThreads, 1)
+    k_lora_pair(const __grid_constant__ LoraMaps maps, LoraSched<NH> sched, Out16Epi epi, ErrorRecord* err,
                 uint64_t timeout_ns) {
   sched.maps = &maps;
   epi.tmC = &maps.y;
-  pair::gemm_core_pair<2>(&maps.x, &maps.w, sched, epi, err, timeout_ns, -1);
+  pair::gemm_core_pair<NH>(&maps.x, &maps.w, sched, epi, err, timeout_ns, -1);
 }
 
 namespace {
@@ -413,6 +472,29 @@ void allow_smem(K kernel, uint32_t bytes, bool* done) {
   GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   if (dev < 64) done[dev] = true;
 }
+constexpr int kRingKb = 112;  // k_lora_split's ring: leaves room for a k_lora_down CTA on the same SM
+
+template <int NH>
+void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, int rc, const TileLists& lists,
+                 cudaStream_t stream) {
+  using Cf = pair::PairCfg<NH>;
+  LoraSched<NH> s;
+  s.T = T;
+  s.N = N;
+  s.K = K;
+  s.rc = rc;
+  s.num_m = (T + kPairRows - 1) / kPairRows;
+  s.num_n = (N + Cf::kCols - 1) / Cf::kCols;
+  s.group_m = ops::gemm_tuning().pair_group_m;
+  s.fmt = e.fmt;
+  s.lists = lists;
+  s.maps = nullptr;
+  static bool done[64] = {false};
+  allow_smem(k_lora_pair<NH>, Cf::kSmemBytesSwizzled, done);
+  const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
+  split::launch_dependent(k_lora_pair<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
+                          device_error_record(), default_timeout_ns());
+}
 }  // namespace
 }  // namespace lora
 
@@ -436,8 +518,10 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   check_rows("work", work, 8, 8);
   if (y == nullptr || ldy < N || adapter == nullptr || scale == nullptr)
     throw std::runtime_error("gicc::lora_linear: y needs rows of at least N elements; adapter and scale are needed");
-  if (tile < 0 || tile > 2) throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split) or 2 (pairs)");
-  if (tile == 0) tile = T <= 256 ? 1 : 2;
+  if (tile < 0 || tile > 3)
+    throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
+  if (tile == 0) tile = split::pick_tile(T, N, K, 1, kRingKb, reinterpret_cast<const void*>(k_lora_split),
+                                         10.0 + (double)T * K * 2 / 4.5e6);
 
   const Work lay = work_layout(T, L, r);
   uint8_t* base = static_cast<uint8_t*>(work);
@@ -455,20 +539,25 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   d.rp = (r + 15) / 16 * 16;
   d.xrows = std::min(split::kRows, (T + 7) / 8 * 8);
   d.fmt = fmt;
-  if (tile == 2) {
+  if (tile != 1) {
     d.lists.count = reinterpret_cast<int*>(base + lay.count);
     d.lists.list = reinterpret_cast<int*>(base + lay.list);
     d.lists.skip = reinterpret_cast<uint32_t*>(base + lay.skip);
     d.lists.cap = lay.cap;
   }
-  // Split K over clusters until about two CTAs per SM work; with few tiles, spread the tiles'
-  // adapters (as many as there may be) over further clusters too.
+  // Many tiles: one CTA per SM with a deep ring (k_lora_pair starts afterwards).  Few: smaller
+  // CTAs, so that k_lora_split's fit beside them, the tiles' adapters (as many as there may be)
+  // spread over further clusters.
+  const int most = std::min(L, std::min(T, split::kRows));
+  const uint32_t ring = tile == 1 ? kDownRing : 2 * kDownRing;
   int S = 1;
-  while (S < split::kMaxSplit && S * 2 <= nkb && tiles * S < 2 * sms) S *= 2;
-  d.groups = std::max(1, std::min(std::min(L, std::min(T, split::kRows)), sms / (tiles * S)));
-  d.stages = std::max(2, std::min<int>(split::kMaxStages, kDownRing / down_stage(d.rp)));
-  const uint32_t dsmem = 1024 + down_ring(d.rp, d.stages) + split::kBarBytes +
-                         (tile == 2 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows>));
+  while (S < 4 && S + 1 <= nkb && tiles * (S + 1) <= sms) ++S;
+  if (tiles == 1 && nkb >= 2 * split::kMaxSplit) S = split::kMaxSplit;  // 33 such clusters fit, two CTAs per SM
+  d.groups = std::max(1, std::min(most, sms / (tiles * S)));
+  d.cap = std::max(1, std::min(kDownCols / d.rp, (most + d.groups - 1) / d.groups));
+  d.stages = std::max(2, std::min<int>(split::kMaxStages, ring / down_stage(d.xrows, d.cap * d.rp)));
+  const uint32_t dsmem = 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) + (kDownBar + 15) / 16 * 16 +
+                         (tile != 1 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows, false>));
   static bool done_down[64] = {false};
   allow_smem(k_lora_down, 227 * 1024, done_down);
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -478,20 +567,21 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
 
   const int rc = (r + BK - 1) / BK;
   if (tile == 1) {
-    const split::Plan p = split::plan(T, N, K, 1, sizeof(LaneLists<split::kRows>));
+    const split::Plan p = split::plan(T, N, K, 1, kRingKb, sizeof(LaneLists<split::kRows>),
+                                        reinterpret_cast<const void*>(k_lora_split));
     LoraSplitOp op;
     op.adapter = adapter;
     op.y = static_cast<uint16_t*>(y);
     op.ldy = ldy;
     op.T = T;
     op.N = N;
+    op.K = K;
     op.L = L;
     op.r = r;
     op.rc = rc;
     op.type = fmt;
     op.vec = (reinterpret_cast<uintptr_t>(y) & 7) == 0 && ldy % 4 == 0;
-    op.bn = p.sh.bn;
-    op.tmV = op.tmB = nullptr;
+    op.tmX = op.tmW = op.tmV = op.tmB = nullptr;
     op.lists = nullptr;
     static bool done[64] = {false};
     allow_smem(k_lora_split, 227 * 1024, done);
@@ -504,7 +594,6 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
         device_error_record(), default_timeout_ns());
     return;
   }
-  using Cf = pair::PairCfg<2>;
   LoraMaps m;
   m.x = make_tmap_2d(x, k16, 2, T, K, ldx, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   m.w = make_tmap_2d(w, k16, 2, N, K, ldw, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -517,23 +606,9 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   e.N = N;
   e.fmt = fmt;
   e.vec = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ldy % 8 == 0;
-  m.y = e.vec ? make_tmap_2d(y, k16, 2, T, N, ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE) : m.x;
-  LoraSched s;
-  s.T = T;
-  s.N = N;
-  s.K = K;
-  s.rc = rc;
-  s.num_m = (T + kPairRows - 1) / kPairRows;
-  s.num_n = (N + Cf::kCols - 1) / Cf::kCols;
-  s.group_m = gemm_tuning().pair_group_m;
-  s.fmt = fmt;
-  s.lists = d.lists;
-  s.maps = nullptr;
-  static bool done[64] = {false};
-  allow_smem(k_lora_pair, Cf::kSmemBytesStaged, done);
-  const int grid = 2 * std::min(s.num_m * s.num_n, sms / 2);
-  k_lora_pair<<<grid, Cf::kThreads, Cf::kSmemBytesStaged, stream>>>(m, s, e, device_error_record(), default_timeout_ns());
-  GICC_CUDA(cudaGetLastError());
+  m.y = e.vec ? make_tmap_2d(y, k16, 2, T, N, ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : m.x;
+  if (tile == 2) launch_pair<2>(m, e, T, N, K, rc, d.lists, stream);
+  else launch_pair<1>(m, e, T, N, K, rc, d.lists, stream);
 }
 
 }  // namespace ops

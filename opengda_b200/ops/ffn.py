@@ -45,28 +45,12 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
 
 def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                           saved: torch.Tensor, act: str = "silu", need_dx: bool = True,
-                          need_dw: bool = True) -> Tuple[Optional[torch.Tensor], ...]:
+                          need_dw: bool = True, tile: int = 0) -> Tuple[Optional[torch.Tensor], ...]:
     """Gradients ``(dx, dw_gate, dw_up)`` of ``gated_linear`` from ``dh`` (row-major) and the
     forward's ``saved``; None for those not wanted.  The gradients of g and u are rounded to the
     inputs' type once, between the activation's derivative and the products; sums are f32."""
-    return native().gated_linear_backward(dh, x, w_gate, w_up, saved, _act(act), bool(need_dx), bool(need_dw))
-
-
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, act):
-        h, saved = gated_linear_forward(x, w_gate, w_up, act)
-        ctx.save_for_backward(x, w_gate, w_up, saved)
-        ctx.act = act
-        return h
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh):
-        x, w_gate, w_up, saved = ctx.saved_tensors
-        need_x, need_g, need_u = ctx.needs_input_grad[:3]
-        dx, dg, du = gated_linear_backward(dh.contiguous(), x, w_gate, w_up, saved, ctx.act, need_x, need_g or need_u)
-        return dx, dg if need_g else None, du if need_u else None, None
+    return native().gated_linear_backward(dh, x, w_gate, w_up, saved, _act(act), bool(need_dx), bool(need_dw),
+                                          int(tile))
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu",
@@ -84,5 +68,5 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         if out is not None or tile:
             raise ValueError("gated_linear: out and tile are for calls without gradients")
-        return _GatedLinear.apply(x, w_gate, w_up, act)
+        return native().gated_linear_autograd(x, w_gate, w_up, _act(act))
     return gated_linear_forward(x, w_gate, w_up, act, save=False, out=out, tile=tile)[0]

@@ -31,7 +31,7 @@ def _sync():
     check_errors()
 
 
-@pytest.mark.parametrize("tile", [1, 2])
+@pytest.mark.parametrize("tile", [1, 2, 3])
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 @pytest.mark.parametrize("T,K,N,L,r,idx", [
     (1, 8, 1, 1, 8, "distinct"), (1, 520, 256, 3, 16, "distinct"), (7, 136, 33, 4, 24, "random"),
