@@ -236,7 +236,9 @@ __device__ __forceinline__ void bulk_wait_read() {
 //                          holds half_n / 2 rows of B, the leader's first
 //   idesc(ti, n), a_desc(ti, addr, k), b_desc(ti, addr, k)  the MMA descriptors of k-step k of a stage
 // and, with `static constexpr bool kLanes = true`,
-//   lane_skip(ti, kb, skip)  true: this k-block leaves the TMEM lanes set in skip[8] alone
+//   lane_skip(ti, kb, skip)  -1: a plain k-block; else it is lane-masked: the number of its
+//                            k-steps, k-step k leaving the TMEM lanes set in skip[k] alone
+//   lane_a_desc(addr, k), lane_b_desc(addr, k)  the descriptors of such a k-step
 template <class S, class = void>
 struct sched_own : std::false_type {};
 template <class S>
@@ -513,7 +515,7 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
         // k-step kb's MMAs for column halves [h0, h1) from the stage that holds it.  The
         // lane-masked form is a loop of its own: beside it in one loop, the plain MMAs were
         // issued too slowly to keep the tensor cores busy.
-        auto issue_mma = [&](auto lanes, const uint32_t* skip, int st, int kb, int h0, int h1) {
+        auto issue_mma = [&](int st, int kb, int h0, int h1) {
           const uint32_t a0 = ptx::smem_u32(sA + st * kABytes);
           const uint32_t b0 = ptx::smem_u32(sB + st * NH * kBBytes);
           uint32_t idesc[NH];
@@ -537,21 +539,30 @@ __device__ __forceinline__ void gemm_core_pair(const CUtensorMap* tmA, const CUt
               uint64_t bd;
               if constexpr (sched_own<Sched>::value) bd = sched.b_desc(ti, b0 + h * kBBytes, k);
               else bd = ptx::sdesc_kmajor_sw128(b0 + h * kBBytes + k * 32);
-              if constexpr (decltype(lanes)::value) mma_pair_lanes(d + h * BN2, ad, bd, idesc[h], 1u, skip);
-              else if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc[h], (kb > ti.kb0 || k > 0) ? 1u : 0u);
+              if constexpr (kTf32) mma_pair_tf32(d + h * BN2, ad, bd, idesc[h], (kb > ti.kb0 || k > 0) ? 1u : 0u);
               else mma_pair(d + h * BN2, ad, bd, idesc[h], (kb > ti.kb0 || k > 0) ? 1u : 0u);
             }
           }
         };
         auto issue = [&](int st, int kb, int h0, int h1) {
           if constexpr (sched_lanes<Sched>::value) {
-            uint32_t skip[8];
-            if (sched.lane_skip(ti, kb, skip)) {
-              issue_mma(std::true_type{}, skip, st, kb, h0, h1);
+            uint32_t skip[BK / 16][8];
+            const int n = sched.lane_skip(ti, kb, skip);  // k-steps of a lane-masked k-block, -1: a plain one
+            if (n >= 0) {
+              const uint32_t a0 = ptx::smem_u32(sA + st * kABytes), b0 = ptx::smem_u32(sB + st * NH * kBBytes);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                  const int cols = sched.half_n(ti, h);
+                  if (h < h0 || h >= h1 || k >= n || cols == 0) continue;
+                  mma_pair_lanes(d + h * BN2, sched.lane_a_desc(a0, k), sched.lane_b_desc(b0 + h * kBBytes, k),
+                                 sched.idesc(ti, cols), 1u, skip[k]);
+                }
               return;
             }
           }
-          issue_mma(std::false_type{}, nullptr, st, kb, h0, h1);
+          issue_mma(st, kb, h0, h1);
         };
         auto release = [&](int st) {
           const uint32_t e_own = ptx::smem_u32(&empty[st]);

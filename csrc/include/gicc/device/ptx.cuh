@@ -400,6 +400,14 @@ __device__ __forceinline__ uint64_t sdesc_kmajor_sw128(uint32_t smem_addr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// The same for rows of `row_bytes` = 32, 64 or 128 bytes with the swizzle of that width (layout 6,
+// 4 or 2): 8-row atoms of 8 * row_bytes.
+__device__ __forceinline__ uint64_t sdesc_kmajor(uint32_t smem_addr, uint32_t row_bytes) {
+  const uint64_t layout = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(row_bytes * 8 >> 4) << 32) |
+         ((uint64_t)1 << 46) | (layout << 61);
+}
+
 // Shared-memory matrix descriptor, MN-major operand, 128-byte swizzle: rows of 128 B hold 64
 // consecutive M (or N) elements of one k; 8 k make a 1024-byte swizzle atom (SBO: the next 8 k),
 // and the next 64 M (or N) elements follow `mn_step` bytes later (LBO).

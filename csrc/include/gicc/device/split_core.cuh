@@ -27,7 +27,7 @@ constexpr int kThreads = 192;
 constexpr int kMaxSplit = 8;            // portable cluster size
 constexpr int kMaxCols = 256;           // columns of all weights per tile (the MMA's N)
 constexpr int kMaxStages = 12;
-constexpr uint32_t kBarBytes = (2 * kMaxStages + 2) * 8 + 16;
+constexpr uint32_t kBarBytes = (2 * kMaxStages + 3) * 8 + 8;
 
 struct Shape {
   int T, N, K;   // rows of X, rows of each W, depth
@@ -85,9 +85,10 @@ __device__ __forceinline__ void store4_16(uint16_t* row, int col, int N, const f
 //   idesc(n), x_desc(addr, k), w_desc(addr, k)  the MMA descriptors of k-step k of a k-block
 //   depth()                        k-blocks
 //   extra_blocks(c, S, e0, e1)     this CTA's further k-blocks after the weights'
-//   extra_wait()                   by the producer before the first of them
-//   extra_loads(e, t0, n0, x, w, bar)         loads of one (as many bytes as a k-block's)
-//   extra_mma(e, d, x, w, idesc)              its MMAs
+//   extra_shared(t0, bar)          by the producer before the first of them: waits for what they
+//                                  need and loads what all share (arrives on bar with its bytes)
+//   extra_loads(e, n0, w, bar)     loads of one (w_bytes)
+//   extra_mma(e, d, w, idesc)      its MMAs
 //   emit(row, col, v)              v[i][4]: four columns of weight i of one valid row
 //   finish()                       by all threads, last
 // The K-major operands and no further k-blocks: the base of most Ops.
@@ -108,9 +109,9 @@ struct PlainOp {
     ptx::tma_load_2d(x, tmX, bar, kb * BK, t0);
   }
   __device__ void extra_blocks(int, int, int& e0, int& e1) const { e0 = e1 = 0; }
-  __device__ void extra_wait() const {}
-  __device__ void extra_loads(int, int, int, uint8_t*, uint8_t*, uint64_t*) const {}
-  __device__ void extra_mma(int, uint32_t, uint32_t, uint32_t, uint32_t) const {}
+  __device__ void extra_shared(int, uint64_t*) const {}
+  __device__ void extra_loads(int, int, uint8_t*, uint64_t*) const {}
+  __device__ void extra_mma(int, uint32_t, uint32_t, uint32_t) const {}
   __device__ void finish() const {}
 };
 
@@ -128,7 +129,8 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* drain = tfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* once = drain + 1;  // what the further k-blocks share has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(once + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* part = reinterpret_cast<float*>(smem);  // after the last MMA: this CTA's partial
 
@@ -149,6 +151,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
     }
     ptx::mbar_init(tfull, 1);
     ptx::mbar_init(drain, 1);
+    ptx::mbar_init(once, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     op.prefetch_maps();
@@ -174,6 +177,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
+      bool shared = false;
       for (int i = 0; i < steps; ++i) {
         if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
           if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
@@ -181,7 +185,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
           break;
         }
         const int b0 = i * group, nb = min(group, blocks - b0);
-        ptx::mbar_arrive_expect_tx(&full[stage], nb * (xb + wb));
+        ptx::mbar_arrive_expect_tx(&full[stage], nb * wb + max(0, min(nb, nk - b0)) * xb);
         for (int j = 0; j < nb; ++j) {
           const int b = b0 + j;
           uint8_t* x = sX + (stage * group + j) * xb;
@@ -189,8 +193,11 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
           if (b < nk) {
             op.loads(kb0 + b, t0, n0, x, w, &full[stage]);
           } else {
-            if (b == nk) op.extra_wait();
-            op.extra_loads(e0 + b - nk, t0, n0, x, w, &full[stage]);
+            if (!shared) {
+              op.extra_shared(t0, once);
+              shared = true;
+            }
+            op.extra_loads(e0 + b - nk, n0, w, &full[stage]);
           }
         }
         issued = i + 1;
@@ -203,6 +210,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
         // Let the TMA loads already issued land before the CTA's smem is used again.
         for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
           ptx::mbar_wait(&full[i % stages], (i / stages) & 1, 20000000ull, nullptr);
+        if (shared) ptx::mbar_wait(once, 0, 20000000ull, nullptr);
       }
     }
     __syncwarp();
@@ -220,6 +228,12 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
         }
         ptx::tc_fence_after();
         const int b0 = i * group, nb = min(group, blocks - b0);
+        if (b0 <= nk && b0 + nb > nk && !ptx::mbar_wait(once, 0, timeout_ns, abort_flag)) {
+          if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 4, 0);
+          *abort_flag = 1;
+          break;
+        }
+        ptx::tc_fence_after();
         for (int j = 0; j < nb; ++j) {
           const uint32_t x = ptx::smem_u32(sX + (stage * group + j) * xb);
           const uint32_t w = ptx::smem_u32(sW + (stage * group + j) * wb);
@@ -228,7 +242,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
             for (int k = 0; k < BK / 16; ++k)
               ptx::mma_f16_ss(tmem, op.x_desc(x, k), op.w_desc(w, k), idesc, (b0 + j > 0 || k > 0) ? 1u : 0u);
           } else {
-            op.extra_mma(e0 + b0 + j - nk, tmem, x, w, idesc);
+            op.extra_mma(e0 + b0 + j - nk, tmem, w, idesc);
           }
         }
         ptx::mma_commit(&empty[stage]);

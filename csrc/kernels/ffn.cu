@@ -174,57 +174,109 @@ __global__ void __launch_bounds__(split::kThreads, 1)
 }
 
 // ---- backward ------------------------------------------------------------------------------
-// One block per 32 rows x 128 columns.  In the saved layout a lane is a row, so g and u come as
-// 512-byte warp loads; dh, dg and du pass through shared memory, so that their global accesses
-// are whole 256-byte row pieces too.  Bound by its 14 bytes per element (saved 8, dh 2, dg and
-// du 4).  The first block also sets the tile counter of k_gated_bwd.
+// Tiles of 32 rows x 128 columns, two persistent blocks per SM.  In the saved layout a lane is a
+// row and a tile's g and u are 16 KB each in one piece: they come by bulk copies into a ring of
+// two, ahead of the arithmetic, and dh one tile ahead into registers; dh, dg and du pass through
+// shared memory so that their global accesses are whole 256-byte row pieces.  Bound by its 14
+// bytes per element (saved 8, dh 2, dg and du 4).  The first block also sets the tile counter of
+// k_gated_bwd.
 constexpr int kGradCols = 128;
 constexpr int kGradPitch = kGradCols + 8;  // 16-bit words: 16-byte accesses of 8 rows on 32 banks
+constexpr uint32_t kGradPlane = 32 * kGradCols * 4;
+constexpr uint32_t kGradBox = 32 * kGradPitch * 2;
+constexpr uint32_t kGradSmem = 2 * 2 * kGradPlane + 3 * kGradBox + 32;
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
     k_gate_grad(const uint16_t* __restrict__ dh, long long lddh, const float* __restrict__ saved,
                 uint16_t* __restrict__ dgu, int T, int I, int Ip, int kind, int fmt, int vec, unsigned int* counter,
-                unsigned int first_tile) {
-  __shared__ alignas(16) uint16_t sd[32 * kGradPitch], so[2][32 * kGradPitch];
+                unsigned int first_tile, ErrorRecord* err, uint64_t timeout_ns) {
+  extern __shared__ __align__(128) uint8_t grad_smem[];
+  uint16_t* sd = reinterpret_cast<uint16_t*>(grad_smem + 4 * kGradPlane);
+  uint16_t* so = sd + kGradBox / 2;  // dg, then du
+  uint64_t* full = reinterpret_cast<uint64_t*>(grad_smem + 4 * kGradPlane + 3 * kGradBox);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + 2);
   ptx::griddep_launch();
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = first_tile;
-  const int i0 = blockIdx.x * kGradCols;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *counter = first_tile;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cols = saved_cols(I);
+  const int tiles_x = (cols + kGradCols - 1) / kGradCols;
+  const long long tiles = (long long)tiles_x * ((T + 31) / 32);
   const size_t plane = saved_plane(T, I), out_plane = (size_t)T * Ip;
-  for (int tb = blockIdx.y; tb < (T + 31) / 32; tb += gridDim.y) {
-    const int t0 = tb * 32, rows = min(32, T - t0);
-    const int t = t0 + lane, i = i0 + warp * 16;
-    const bool work = lane < rows && i < saved_cols(I);
-    uint4 gv[4], uv[4];
-    if (work) {
-      const float* gp = saved + saved_at(t, i, I);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        gv[j] = ptx::ld_v4_nc(gp + 128 * j);
-        uv[j] = ptx::ld_v4_nc(gp + plane + 128 * j);
-      }
-    }
+  if (tid == 0) {
+    ptx::mbar_init(&full[0], 1);
+    ptx::mbar_init(&full[1], 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  auto load_saved = [&](long long tile, int stage) {  // by one thread
+    const int i0 = (int)(tile % tiles_x) * kGradCols;
+    const float* g = saved + saved_at((int)(tile / tiles_x) * 32, i0, I);
+    const uint32_t bytes = min(kGradCols, cols - i0) * 128;
+    ptx::mbar_arrive_expect_tx(&full[stage], 2 * bytes);
+    ptx::bulk_load(grad_smem + stage * 2 * kGradPlane, g, bytes, &full[stage]);
+    ptx::bulk_load(grad_smem + (stage * 2 + 1) * kGradPlane, g + plane, bytes, &full[stage]);
+  };
+  uint16_t pre[16];
+  auto load_dh = [&](long long tile) {
+    const int t0 = (int)(tile / tiles_x) * 32, i0 = (int)(tile % tiles_x) * kGradCols;
+    const int rows = min(32, T - t0);
     if (vec) {
-      for (int q = threadIdx.x; q < 32 * (kGradCols / 8); q += 256) {
-        const int r = q / (kGradCols / 8), col = q % (kGradCols / 8) * 8;
-        if (r >= rows || i0 + col >= I) continue;
-        const uint16_t* p = dh + (size_t)(t0 + r) * lddh + i0 + col;
-        uint16_t* d = sd + r * kGradPitch + col;
-        if (i0 + col + 8 <= I) {
-          *reinterpret_cast<uint4*>(d) = ptx::ld_v4_nc(p);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int q = tid + k * 256, r = q / (kGradCols / 8), i = i0 + q % (kGradCols / 8) * 8;
+        const uint16_t* p = dh + (size_t)(t0 + r) * lddh + i;
+        if (r < rows && i + 8 <= I) {
+          *reinterpret_cast<uint4*>(pre + 8 * k) = ptx::ld_v4_nc(p);
         } else {
-          for (int k = 0; i0 + col + k < I; ++k) d[k] = p[k];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pre[8 * k + e] = r < rows && i + e < I ? p[e] : (uint16_t)0;
         }
       }
     } else {
-#pragma unroll 8
-      for (int q = threadIdx.x; q < 32 * kGradCols; q += 256) {
-        const int r = q / kGradCols, col = q % kGradCols;
-        if (r < rows && i0 + col < I) sd[r * kGradPitch + col] = dh[(size_t)(t0 + r) * lddh + i0 + col];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int q = tid + k * 256, r = q / kGradCols, i = i0 + q % kGradCols;
+        pre[k] = r < rows && i < I ? dh[(size_t)(t0 + r) * lddh + i] : (uint16_t)0;
       }
     }
+  };
+  long long tile = blockIdx.x;
+  if (tile < tiles) {
+    if (tid == 0) {
+      load_saved(tile, 0);
+      if (tile + gridDim.x < tiles) load_saved(tile + gridDim.x, 1);
+    }
+    load_dh(tile);
+  }
+  for (int it = 0; tile < tiles; tile += gridDim.x, ++it) {
+    const int stage = it & 1;
+    const int t0 = (int)(tile / tiles_x) * 32, i0 = (int)(tile % tiles_x) * kGradCols;
+    const int rows = min(32, T - t0);
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int q = tid + k * 256;
+        *reinterpret_cast<uint4*>(sd + q / (kGradCols / 8) * kGradPitch + q % (kGradCols / 8) * 8) =
+            *reinterpret_cast<const uint4*>(pre + 8 * k);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int q = tid + k * 256;
+        sd[q / kGradCols * kGradPitch + q % kGradCols] = pre[k];
+      }
+    }
+    if (tile + gridDim.x < tiles) load_dh(tile + gridDim.x);
+    if (!ptx::mbar_wait(&full[stage], (it >> 1) & 1, timeout_ns, abort_flag)) {
+      if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
+      *abort_flag = 1;
+    }
     __syncthreads();
-    if (work) {
+    if (*abort_flag) break;
+    const int i = i0 + warp * 16;
+    if (lane < rows && i < cols) {
+      const uint4* gp = reinterpret_cast<const uint4*>(grad_smem + stage * 2 * kGradPlane) + warp * 128 + lane;
       const uint4* dp = reinterpret_cast<const uint4*>(sd + lane * kGradPitch + warp * 16);
       uint16_t d[16];
       *reinterpret_cast<uint4*>(d) = dp[0];
@@ -232,12 +284,12 @@ __global__ void __launch_bounds__(256)
       uint32_t og[8], ou[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float g[4] = {__uint_as_float(gv[j].x), __uint_as_float(gv[j].y), __uint_as_float(gv[j].z), __uint_as_float(gv[j].w)};
-        const float u[4] = {__uint_as_float(uv[j].x), __uint_as_float(uv[j].y), __uint_as_float(uv[j].z), __uint_as_float(uv[j].w)};
+        const uint4 gv = gp[32 * j], uv = gp[32 * j + kGradPlane / 16];
+        const float g[4] = {__uint_as_float(gv.x), __uint_as_float(gv.y), __uint_as_float(gv.z), __uint_as_float(gv.w)};
+        const float u[4] = {__uint_as_float(uv.x), __uint_as_float(uv.y), __uint_as_float(uv.z), __uint_as_float(uv.w)};
         float a[4], e[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          // columns past I (never read back) hold whatever the tile held before
           const float dv = ptx::from_16(d[4 * j + k], fmt);
           float slope;
           a[k] = dv * act::value_grad(g[k], kind, &slope);
@@ -248,21 +300,29 @@ __global__ void __launch_bounds__(256)
         ou[2 * j] = ptx::pack_16x2(a[0], a[1], fmt);
         ou[2 * j + 1] = ptx::pack_16x2(a[2], a[3], fmt);
       }
-      uint4* pg = reinterpret_cast<uint4*>(so[0] + lane * kGradPitch + warp * 16);
-      uint4* pu = reinterpret_cast<uint4*>(so[1] + lane * kGradPitch + warp * 16);
+      uint4* pg = reinterpret_cast<uint4*>(so + lane * kGradPitch + warp * 16);
+      uint4* pu = reinterpret_cast<uint4*>(so + kGradBox / 2 + lane * kGradPitch + warp * 16);
       pg[0] = make_uint4(og[0], og[1], og[2], og[3]);
       pg[1] = make_uint4(og[4], og[5], og[6], og[7]);
       pu[0] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
       pu[1] = make_uint4(ou[4], ou[5], ou[6], ou[7]);
     }
     __syncthreads();
-    for (int q = threadIdx.x; q < 2 * 32 * (kGradCols / 8); q += 256) {
-      const int z = q / (32 * (kGradCols / 8)), r = q / (kGradCols / 8) % 32, col = q % (kGradCols / 8) * 8;
-      if (r < rows && i0 + col < saved_cols(I))  // saved_cols(I) <= Ip
+    if (tid == 0 && tile + 2 * (long long)gridDim.x < tiles) load_saved(tile + 2 * (long long)gridDim.x, stage);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int q = tid + k * 256, z = q / 512, r = q / (kGradCols / 8) % 32, col = q % (kGradCols / 8) * 8;
+      if (r < rows && i0 + col < cols)  // cols <= Ip
         ptx::st_v4(dgu + z * out_plane + (size_t)(t0 + r) * Ip + i0 + col,
-                   *reinterpret_cast<const uint4*>(so[z] + r * kGradPitch + col));
+                   *reinterpret_cast<const uint4*>(so + z * (kGradBox / 2) + r * kGradPitch + col));
     }
   }
+  // An aborted block lets the copies it has issued land before its shared memory goes.
+  if (*abort_flag && tid == 0)
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_wait(&full[s], 0, 20000000ull, nullptr);
+      ptx::mbar_wait(&full[s], 1, 20000000ull, nullptr);
+    }
 }
 
 struct BwdMaps {
@@ -654,9 +714,13 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   const BwdPlan plan = plan_bwd(T, H, I, dx != nullptr, dw_gate != nullptr, tile);
   uint16_t* dgu = static_cast<uint16_t*>(work);
   unsigned int* counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(work) + grad_counter_at(T, I));
-  const dim3 ggrid((saved_cols(I) + kGradCols - 1) / kGradCols, std::min((T + 31) / 32, 32768));
-  k_gate_grad<<<ggrid, 256, 0, stream>>>(static_cast<const uint16_t*>(dh), lddh, saved, dgu, T, I, Ip, kind, fmt,
-                                         vec16(dh, lddh) ? 1 : 0, counter, (unsigned)(num_sms() / 2));
+  const long long gtiles = (long long)((saved_cols(I) + kGradCols - 1) / kGradCols) * ((T + 31) / 32);
+  const int ggrid = (int)std::min<long long>(gtiles, 2LL * num_sms());
+  static bool grad_done[64] = {false};
+  allow_smem(k_gate_grad, kGradSmem, grad_done);
+  k_gate_grad<<<ggrid, 256, kGradSmem, stream>>>(static_cast<const uint16_t*>(dh), lddh, saved, dgu, T, I, Ip, kind, fmt,
+                                                 vec16(dh, lddh) ? 1 : 0, counter, (unsigned)(num_sms() / 2),
+                                                 device_error_record(), default_timeout_ns());
   GICC_CUDA(cudaGetLastError());
 
   BwdMaps m;

@@ -10,7 +10,10 @@
 // every adapter to its own rows (adapter_lanes.cuh).  So rows keep their order, the product
 // with B[a] costs no pass of its own over y, and a row without an adapter gets W x alone.
 // v is rounded to 16 bits, as an MMA operand must be; it enters y only through the adapter's
-// term.  A tile pays one k-block (64 deep) per adapter it meets, r <= 64.
+// term.  A k-block holds 64 / w pieces of w = 16, 32 or 64 columns (the largest that divides r),
+// each a piece of one adapter of the tile, with the swizzle of its width: pieces as wide as r,
+// because TMA fills the missing columns of a wider box slowly (1.7 us a block at r = 16 in boxes
+// of 64 columns, against 0.7 us at r = 64).
 //
 // Few rows: the split-K cluster core (k_lora_split); it starts while k_lora_down still runs and
 // waits for v only before its adapter blocks.  Many rows: the CTA-pair core (k_lora_pair), whose
@@ -43,6 +46,24 @@ struct TileLists {
   int cap = 0;               // min(L, 256)
 };
 
+// How an adapter's r columns are cut into pieces of one width, and those into k-blocks.
+struct Pieces {
+  int w;      // columns of a piece: 64, 32 or 16
+  int each;   // pieces of an adapter
+  int block;  // pieces in a k-block
+  __host__ __device__ int blocks(int adapters) const { return (adapters * each + block - 1) / block; }
+};
+inline Pieces pieces(int r) {
+  Pieces p;
+  p.w = r % 64 == 0 ? 64 : r % 32 == 0 ? 32 : 16;
+  p.each = (r + p.w - 1) / p.w;
+  p.block = BK / p.w;
+  return p;
+}
+inline CUtensorMapSwizzle piece_swizzle(const Pieces& p) {
+  return p.w == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : p.w == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+}
+
 // ---- v = s A x ---------------------------------------------------------------------------------
 // Grid (S, G, ceil(T / 128)): a cluster of S CTAs splits K for one 128-row tile and the adapters
 // i with i % G == blockIdx.y of the tile's list (one group when there are many tiles).  The
@@ -67,6 +88,7 @@ struct DownArgs {
 constexpr int kDownCols = 128;  // columns of an accumulator
 // Beside a k_lora_split CTA's ring both fit an SM.
 constexpr uint32_t kDownRing = 92 * 1024;
+constexpr uint32_t kDownMin = 116 * 1024;
 __host__ __device__ constexpr uint32_t down_stage(int xrows, int cols) { return split::x_bytes(xrows) + cols * BK * 2; }
 // as split::ring_bytes: the MMA reads 128 rows from the last x box on
 __host__ __device__ constexpr uint32_t down_ring(int rp, int cols, int xrows, int stages) {
@@ -314,32 +336,64 @@ struct LoraSplitOp : split::PlainOp {
   const int* adapter;
   uint16_t* y;
   long long ldy;
-  int T, N, K, L, r, rc;  // rc: k-blocks of 64 per adapter
+  int T, N, K, L;
+  Pieces pc;
   int vec;
+  uint32_t xpiece, wpiece;  // bytes of a piece of v and of B
   const CUtensorMap* tmV;  // set by the kernel
   const CUtensorMap* tmB;
   const LaneLists<split::kRows>* lists;
   __device__ int depth() const { return (K + BK - 1) / BK; }
+  uint8_t* sV;  // the tile's rows of v, piece by piece, loaded once: every CTA of the grid reads them
   __device__ void prepare(uint8_t* smem, int t0, ErrorRecord*) {
-    auto* l = reinterpret_cast<LaneLists<split::kRows>*>(smem);
+    sV = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~uintptr_t(1023));
+    auto* l = reinterpret_cast<LaneLists<split::kRows>*>(sV + v_bytes());
     l->build(adapter, t0, T, L, nullptr);  // k_lora_down reports indexes out of range
     lists = l;
   }
+  // The MMA reads 128 rows of the last piece too; its rows behind the box are the lists.
+  __host__ __device__ uint32_t v_bytes() const { return pc.each * xpiece; }
+  __host__ static uint32_t extra_smem(const Pieces& pc, int xrows) {
+    return 1024 + std::max<uint32_t>(pc.each * xrows * pc.w * 2 + sizeof(LaneLists<split::kRows>),
+                                     (pc.each - 1) * xrows * pc.w * 2 + split::kRows * pc.w * 2);
+  }
   __device__ void extra_blocks(int c, int S, int& e0, int& e1) const {
-    const int n = lists->n * rc;
+    const int n = pc.blocks(lists->n);
     e0 = n * c / S;
     e1 = n * (c + 1) / S;
   }
-  __device__ void extra_wait() const { ptx::griddep_wait(); }
-  __device__ void extra_loads(int e, int t0, int n0, uint8_t* sX, uint8_t* sW, uint64_t* bar) const {
-    const int s = e / rc, k = (e - s * rc) * BK;
-    ptx::tma_load_2d(sX, tmV, bar, k, t0);
-    ptx::tma_load_3d(sW, tmB, bar, k, n0, lists->list[s]);
+  __device__ void extra_shared(int t0, uint64_t* bar) const {
+    ptx::griddep_wait();
+    ptx::mbar_arrive_expect_tx(bar, v_bytes());
+    for (int i = 0; i < pc.each; ++i) ptx::tma_load_2d(sV + i * xpiece, tmV, bar, i * pc.w, t0);
   }
-  __device__ void extra_mma(int e, uint32_t d, uint32_t x, uint32_t w, uint32_t idesc) const {
-    const int s = e / rc, left = r - (e - s * rc) * BK;
-    for (int k = 0; k < BK / 16 && k * 16 < left; ++k)
-      ptx::mma_f16_ss_lanes(d, x_desc(x, k), w_desc(w, k), idesc, 1u, lists->skip[s]);
+  __device__ void extra_loads(int e, int n0, uint8_t* sW, uint64_t* bar) const {
+    for (int j = 0; j < pc.block; ++j) {
+      // behind the last piece the last once more: every k-block has the same bytes
+      const int s = min(e * pc.block + j, lists->n * pc.each - 1), i = s / pc.each, k = (s - i * pc.each) * pc.w;
+      ptx::tma_load_3d(sW + j * wpiece, tmB, bar, k, n0, lists->list[i]);
+    }
+  }
+  // Unrolled for each width: the issuing thread is what bounds these short MMAs.
+  template <int W>
+  __device__ __forceinline__ void piece_mma(int e, uint32_t d, uint32_t w, uint32_t idesc) const {
+    const int left = lists->n * pc.each - e * (BK / W);
+    const uint64_t v0 = ptx::sdesc_kmajor(ptx::smem_u32(sV), W * 2), w0 = ptx::sdesc_kmajor(w, W * 2);
+#pragma unroll
+    for (int j = 0; j < BK / W; ++j) {
+      if (j >= left) break;
+      const int s = e * (BK / W) + j, i = pc.each == 1 ? s : s / pc.each, part = s - i * pc.each;
+      const uint4 m = *reinterpret_cast<const uint4*>(lists->skip[i]);
+      const uint32_t skip[4] = {m.x, m.y, m.z, m.w};
+      const uint64_t vd = v0 + ((part * xpiece) >> 4), wd = w0 + ((j * wpiece) >> 4);  // start addresses, 16 bytes
+#pragma unroll
+      for (int k = 0; k < W / 16; ++k) ptx::mma_f16_ss_lanes(d, vd + 2 * k, wd + 2 * k, idesc, 1u, skip);
+    }
+  }
+  __device__ void extra_mma(int e, uint32_t d, uint32_t w, uint32_t idesc) const {
+    if (pc.w == 16) piece_mma<16>(e, d, w, idesc);
+    else if (pc.w == 32) piece_mma<32>(e, d, w, idesc);
+    else piece_mma<64>(e, d, w, idesc);
   }
   __device__ __forceinline__ void emit(int t, int col, const float (*v)[4]) const {
     split::store4_16(y + (size_t)t * ldy, col, N, v[0], type, vec);
@@ -370,7 +424,8 @@ struct LoraSched {
   static constexpr bool kOwnOperands = true;
   static constexpr bool kLanes = true;
   static constexpr bool kDependent = true;
-  int T, N, K, rc;
+  int T, N, K;
+  Pieces pc;
   int num_m, num_n, group_m;
   int fmt;
   TileLists lists;
@@ -386,9 +441,10 @@ struct LoraSched {
     ti.a_row = ti.m0;
     ti.b_row = ti.n0;
     ti.kb0 = 0;
-    ti.kb1 = weight_blocks() + (int)ptx::ld_cg(lists.count + mb) * rc;
+    const int n = (int)ptx::ld_cg(lists.count + mb);
+    ti.kb1 = weight_blocks() + pc.blocks(n);
     ti.aux = mb * lists.cap;
-    ti.aux2 = 0;
+    ti.aux2 = n * pc.each;  // pieces
     return ti;
   }
   __device__ bool producer_wait(const TileInfo&, int, uint64_t, volatile int*, ErrorRecord*) const { return true; }
@@ -401,11 +457,14 @@ struct LoraSched {
       pair::tma_load_2d_pair(sB, &maps->w, bar, kb * BK, n);
       if constexpr (NH == 2) pair::tma_load_2d_pair(sB + pair::kBBytes, &maps->w, bar, kb * BK, n1);
     } else {
-      const int s = e / rc, k = (e - s * rc) * BK;
-      const int a = (int)ptx::ld_cg(lists.list + ti.aux + s);
-      pair::tma_load_2d_pair(sA, &maps->v, bar, k, m);
-      pair::tma_load_3d_pair(sB, &maps->b, bar, k, n, a);
-      if constexpr (NH == 2) pair::tma_load_3d_pair(sB + pair::kBBytes, &maps->b, bar, k, n1, a);
+      const uint32_t bytes = BM * pc.w * 2;
+      for (int j = 0; j < pc.block; ++j) {
+        const int s = min(e * pc.block + j, ti.aux2 - 1), i = s / pc.each, k = (s - i * pc.each) * pc.w;
+        const int a = (int)ptx::ld_cg(lists.list + ti.aux + i);
+        pair::tma_load_2d_pair(sA + j * bytes, &maps->v, bar, k, m);
+        pair::tma_load_3d_pair(sB + j * bytes, &maps->b, bar, k, n, a);
+        if constexpr (NH == 2) pair::tma_load_3d_pair(sB + pair::kBBytes + j * bytes, &maps->b, bar, k, n1, a);
+      }
     }
   }
   __device__ int half_n(const TileInfo& ti, int h) const {
@@ -414,21 +473,33 @@ struct LoraSched {
   __device__ uint32_t idesc(const TileInfo&, int n) const { return ptx::idesc_f16_f32(2 * BM, n, fmt, 0, 0); }
   __device__ uint64_t a_desc(const TileInfo&, uint32_t a, int k) const { return ptx::sdesc_kmajor_sw128(a + k * 32); }
   __device__ uint64_t b_desc(const TileInfo&, uint32_t b, int k) const { return ptx::sdesc_kmajor_sw128(b + k * 32); }
-  __device__ bool lane_skip(const TileInfo& ti, int kb, uint32_t* skip) const {
+  __device__ int lane_skip(const TileInfo& ti, int kb, uint32_t (*skip)[8]) const {
     const int e = kb - weight_blocks();
-    if (e < 0) return false;
-    const uint4* p = reinterpret_cast<const uint4*>(lists.skip + (size_t)(ti.aux + e / rc) * 8);
-    const uint4 a = ptx::ld_v4_cg(p), b = ptx::ld_v4_cg(p + 1);
-    skip[0] = a.x;
-    skip[1] = a.y;
-    skip[2] = a.z;
-    skip[3] = a.w;
-    skip[4] = b.x;
-    skip[5] = b.y;
-    skip[6] = b.z;
-    skip[7] = b.w;
-    return true;
+    if (e < 0) return -1;
+    const int steps = pc.w / 16;  // k-steps of a piece
+    const int n = min(pc.block, ti.aux2 - e * pc.block) * steps;
+#pragma unroll
+    for (int k = 0; k < BK / 16; ++k) {
+      const int s = min(e * pc.block + k / steps, ti.aux2 - 1);
+      const uint4* p = reinterpret_cast<const uint4*>(lists.skip + (size_t)(ti.aux + s / pc.each) * 8);
+      const uint4 a = ptx::ld_v4_cg(p), b = ptx::ld_v4_cg(p + 1);
+      skip[k][0] = a.x;
+      skip[k][1] = a.y;
+      skip[k][2] = a.z;
+      skip[k][3] = a.w;
+      skip[k][4] = b.x;
+      skip[k][5] = b.y;
+      skip[k][6] = b.z;
+      skip[k][7] = b.w;
+    }
+    return n;
   }
+  __device__ uint64_t piece_desc(uint32_t addr, int k) const {
+    const int steps = pc.w / 16, j = k / steps;
+    return ptx::sdesc_kmajor(addr + j * BM * pc.w * 2 + (k - j * steps) * 32, pc.w * 2);
+  }
+  __device__ uint64_t lane_a_desc(uint32_t a, int k) const { return piece_desc(a, k); }
+  __device__ uint64_t lane_b_desc(uint32_t b, int k) const { return piece_desc(b, k); }
 };
 
 template <int NH>
@@ -472,17 +543,17 @@ void allow_smem(K kernel, uint32_t bytes, bool* done) {
   GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   if (dev < 64) done[dev] = true;
 }
-constexpr int kRingKb = 112;  // k_lora_split's ring: leaves room for a k_lora_down CTA on the same SM
+constexpr int kRingKb = 104;  // k_lora_split's ring: leaves room for a k_lora_down CTA on the same SM
 
 template <int NH>
-void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, int rc, const TileLists& lists,
+void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, const Pieces& pc, const TileLists& lists,
                  cudaStream_t stream) {
   using Cf = pair::PairCfg<NH>;
   LoraSched<NH> s;
   s.T = T;
   s.N = N;
   s.K = K;
-  s.rc = rc;
+  s.pc = pc;
   s.num_m = (T + kPairRows - 1) / kPairRows;
   s.num_n = (N + Cf::kCols - 1) / Cf::kCols;
   s.group_m = ops::gemm_tuning().pair_group_m;
@@ -552,12 +623,14 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   const uint32_t ring = tile == 1 ? kDownRing : 2 * kDownRing;
   int S = 1;
   while (S < 4 && S + 1 <= nkb && tiles * (S + 1) <= sms) ++S;
-  if (tiles == 1 && nkb >= 2 * split::kMaxSplit) S = split::kMaxSplit;  // 33 such clusters fit, two CTAs per SM
-  d.groups = std::max(1, std::min(most, sms / (tiles * S)));
+  if (tiles == 1 && nkb >= 2 * split::kMaxSplit) S = split::kMaxSplit;
+  d.groups = std::max(1, std::min(most, split::clusters_at_once(reinterpret_cast<const void*>(k_lora_down), S) / tiles));
   d.cap = std::max(1, std::min(kDownCols / d.rp, (most + d.groups - 1) / d.groups));
   d.stages = std::max(2, std::min<int>(split::kMaxStages, ring / down_stage(d.xrows, d.cap * d.rp)));
-  const uint32_t dsmem = 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) + (kDownBar + 15) / 16 * 16 +
-                         (tile != 1 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows, false>));
+  // at least more than half of an SM's: two of these CTAs on one SM would keep k_lora_split's off it
+  const uint32_t dsmem = std::max<uint32_t>(kDownMin, 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) +
+                                                          (kDownBar + 15) / 16 * 16 +
+                                                          (tile != 1 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows, false>)));
   static bool done_down[64] = {false};
   allow_smem(k_lora_down, 227 * 1024, done_down);
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -565,10 +638,10 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
                          make_tmap_2d(x, k16, 2, T, K, ldx, d.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B), tA, d,
                          device_error_record(), default_timeout_ns());
 
-  const int rc = (r + BK - 1) / BK;
+  const Pieces pc = pieces(r);
   if (tile == 1) {
-    const split::Plan p = split::plan(T, N, K, 1, kRingKb, sizeof(LaneLists<split::kRows>),
-                                        reinterpret_cast<const void*>(k_lora_split));
+    split::Plan p = split::plan(T, N, K, 1, kRingKb, 0, reinterpret_cast<const void*>(k_lora_split));
+    p.smem += LoraSplitOp::extra_smem(pc, p.sh.xrows);
     LoraSplitOp op;
     op.adapter = adapter;
     op.y = static_cast<uint16_t*>(y);
@@ -577,28 +650,30 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
     op.N = N;
     op.K = K;
     op.L = L;
-    op.r = r;
-    op.rc = rc;
+    op.pc = pc;
+    op.xpiece = p.sh.xrows * pc.w * 2;
+    op.wpiece = p.sh.bn * pc.w * 2;
     op.type = fmt;
     op.vec = (reinterpret_cast<uintptr_t>(y) & 7) == 0 && ldy % 4 == 0;
     op.tmX = op.tmW = op.tmV = op.tmB = nullptr;
     op.lists = nullptr;
+    op.sV = nullptr;
     static bool done[64] = {false};
     allow_smem(k_lora_split, 227 * 1024, done);
     split::launch_clusters(
         k_lora_split, p.grid, p.splits, split::kThreads, p.smem, true, stream,
         make_tmap_2d(x, k16, 2, T, K, ldx, p.sh.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B),
         make_tmap_2d(w, k16, 2, N, K, ldw, p.sh.bn, BK, CU_TENSOR_MAP_SWIZZLE_128B),
-        make_tmap_2d(d.v, k16, 2, T, r, r, p.sh.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B),
-        make_tmap_3d(lora_b, k16, 2, L, N, r, r, (uint64_t)N * r, p.sh.bn, BK, CU_TENSOR_MAP_SWIZZLE_128B), p.sh, op,
+        make_tmap_2d(d.v, k16, 2, T, r, r, p.sh.xrows, pc.w, piece_swizzle(pc)),
+        make_tmap_3d(lora_b, k16, 2, L, N, r, r, (uint64_t)N * r, p.sh.bn, pc.w, piece_swizzle(pc)), p.sh, op,
         device_error_record(), default_timeout_ns());
     return;
   }
   LoraMaps m;
   m.x = make_tmap_2d(x, k16, 2, T, K, ldx, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   m.w = make_tmap_2d(w, k16, 2, N, K, ldw, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
-  m.v = make_tmap_2d(d.v, k16, 2, T, r, r, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
-  m.b = make_tmap_3d(lora_b, k16, 2, L, N, r, r, (uint64_t)N * r, BM, BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  m.v = make_tmap_2d(d.v, k16, 2, T, r, r, BM, pc.w, piece_swizzle(pc));
+  m.b = make_tmap_3d(lora_b, k16, 2, L, N, r, r, (uint64_t)N * r, BM, pc.w, piece_swizzle(pc));
   Out16Epi e;
   e.C = static_cast<uint16_t*>(y);
   e.ldc = ldy;
@@ -607,8 +682,8 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   e.fmt = fmt;
   e.vec = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ldy % 8 == 0;
   m.y = e.vec ? make_tmap_2d(y, k16, 2, T, N, ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : m.x;
-  if (tile == 2) launch_pair<2>(m, e, T, N, K, rc, d.lists, stream);
-  else launch_pair<1>(m, e, T, N, K, rc, d.lists, stream);
+  if (tile == 2) launch_pair<2>(m, e, T, N, K, pc, d.lists, stream);
+  else launch_pair<1>(m, e, T, N, K, pc, d.lists, stream);
 }
 
 }  // namespace ops
