@@ -1,6 +1,5 @@
 // module.cpp -- pybind11/torch binding of libgicc (opengda_b200._C).
 // Tensors are validated here; the kernels themselves live in libgicc.so.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -92,12 +91,31 @@ void check_rows(const at::Tensor& t, const char* name, const at::Tensor& like) {
 // The row pitch; a single row's stride says nothing, so it counts as dense.
 long long pitch_of(const at::Tensor& t) { return t.size(0) <= 1 ? std::max<int64_t>((t.size(1) + 7) / 8 * 8, 8) : t.stride(0); }
 
+// Whether `out` (row-major matrix) may share memory with `in`: their address ranges meet, and they
+// are not column ranges of one buffer that lie side by side.
+bool may_overlap(const at::Tensor& out, const at::Tensor& in) {
+  auto bytes = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * (int64_t)t.element_size();
+  };
+  if (out.numel() == 0 || in.numel() == 0) return false;
+  const char *a = static_cast<const char*>(out.data_ptr()), *b = static_cast<const char*>(in.data_ptr());
+  if (a + bytes(out) <= b || b + bytes(in) <= a) return false;
+  if (out.dim() == 2 && in.dim() == 2 && out.size(0) > 1 && in.size(0) > 1 && out.stride(0) == in.stride(0)) {
+    const int64_t pitch = out.stride(0) * (int64_t)out.element_size();
+    const int64_t at = ((a - b) % pitch + pitch) % pitch;  // out's first byte within a row of in's
+    return at < in.size(1) * (int64_t)in.element_size() || at + out.size(1) * (int64_t)out.element_size() > pitch;
+  }
+  return true;
+}
+
 at::Tensor out_or_empty(const c10::optional<at::Tensor>& out, int64_t rows, int64_t cols, const at::Tensor& like,
                         std::initializer_list<at::Tensor> inputs) {
   if (!out.has_value()) return at::empty({rows, cols}, like.options());
   check_rows(*out, "out", like);
   TORCH_CHECK(out->size(0) == rows && out->size(1) == cols, "out has the wrong shape");
-  for (const auto& t : inputs) at::assert_no_overlap(*out, t);
+  for (const auto& t : inputs) TORCH_CHECK(!may_overlap(*out, t), "out must not overlap an input");
   return *out;
 }
 
@@ -179,7 +197,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     if (at::GradMode::is_enabled()) {  // create_graph: there is no second derivative to go through
       torch::autograd::variable_list defined;
       for (const auto& t : out)
-        if (t.defined()) defined.push_back(t);
+        if (t.defined()) defined.push_back(t.detach().requires_grad_(true));
       torch::autograd::DelayedError error("gated_linear: the backward pass is not differentiable", defined.size());
       defined = error.apply(std::move(defined));
       size_t k = 0;
@@ -213,21 +231,21 @@ at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const at::Tenso
                   adapter.size(0) == T && adapter.is_contiguous(),
               "adapter must be a contiguous int32 tensor with one index per row of x, on its device");
   const c10::cuda::CUDAGuard g(x.device());
-  at::Tensor s;
+  const float* sp = nullptr;
   if (scale.has_value()) {
-    s = *scale;
+    const at::Tensor& s = *scale;
     TORCH_CHECK(s.is_cuda() && s.device() == x.device() && s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == L &&
                     s.is_contiguous(),
                 "scale must be a contiguous float32 tensor with one factor per adapter, on x's device");
-  } else {
-    s = at::ones({L}, x.options().dtype(at::kFloat));
+    sp = s.data_ptr<float>();
   }
-  at::Tensor y = out_or_empty(out, T, N, x, {x, w, lora_a, lora_b, adapter, s});
+  at::Tensor y = out_or_empty(out, T, N, x, {x, w, lora_a, lora_b, adapter});
+  TORCH_CHECK(!out.has_value() || !scale.has_value() || !may_overlap(y, *scale), "out must not overlap an input");
   TORCH_CHECK(L >= 1 && r >= 1, "at least one adapter of rank 8 or more");
   if (T > 0) {
     at::Tensor work = at::empty({(int64_t)gicc::ops::lora_work_bytes((int)T, (int)L, (int)r)}, x.options().dtype(at::kByte));
     gicc::ops::lora_linear(x.data_ptr(), w.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), adapter.data_ptr<int>(),
-                           s.data_ptr<float>(), y.data_ptr(), work.data_ptr(), (int)T, (int)K, (int)N, (int)L, (int)r,
+                           sp, y.data_ptr(), work.data_ptr(), (int)T, (int)K, (int)N, (int)L, (int)r,
                            pitch_of(x), pitch_of(w), T == 1 ? std::max<int64_t>(N, y.stride(0)) : y.stride(0), fmt, (int)tile,
                            cur_stream());
   }

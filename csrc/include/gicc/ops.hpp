@@ -68,7 +68,7 @@ GICC_EXPORT void gated_linear_backward(const void* dh, const void* x, const void
 // ---- projection with low-rank adapters (lora.cu) ----------------------------------------------
 // y[t] = W x[t] + scale[a] B[a] (A[a] x[t]), a = adapter[t] (-1: none): x [T, K], W [N, K],
 // A [L, r, K], B [L, N, r] (dense), y [T, N], all f16 (fmt 0) or all bf16 (fmt 1); adapter
-// int32 [T], scale f32 [L].  K % 8 == 0, r % 8 == 0, r <= 128, L <= 8192.  work holds
+// int32 [T], scale f32 [L] or null (1).  K % 8 == 0, r % 8 == 0, r <= 128, L <= 8192.  work holds
 // lora_work_bytes(T, L, r).  tile as for gated_linear.
 GICC_EXPORT size_t lora_work_bytes(int T, int L, int r);
 GICC_EXPORT void lora_linear(const void* x, const void* w, const void* lora_a, const void* lora_b, const int* adapter,

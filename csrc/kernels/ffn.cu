@@ -22,7 +22,11 @@
 // (k_gated_bwd) runs the tiles of all three products: dx over the 2I deep concatenation of
 // [dg | du] and [Wg ; Wu], and the two weight gradients over T.  The MMA reads operands of
 // either major, so nothing is transposed in memory; putting the products into one launch
-// leaves one partly filled last wave instead of two.
+// leaves one partly filled last wave instead of two.  Products with few tiles for that (dx of few
+// rows, small weight gradients over many) go to the split-K cluster core instead.
+//
+// Host entry points: gicc::ops::gated_linear, gated_linear_backward (C++, throw) and
+// gicc_gated_linear, gicc_gated_linear_backward (C ABI).
 #include <algorithm>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -774,3 +778,20 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
 
 }  // namespace ops
 }  // namespace gicc
+
+GICC_API int gicc_gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I,
+                               long long ldx, long long ldg, long long ldu, long long ldh, int kind, int fmt, float* saved,
+                               cudaStream_t stream) {
+  return gicc::guarded([&] {
+    gicc::ops::gated_linear(x, w_gate, w_up, h, T, H, I, ldx, ldg, ldu, ldh, kind, fmt, saved, 0, stream);
+  });
+}
+GICC_API int gicc_gated_linear_backward(const void* dh, const void* x, const void* w_gate, const void* w_up,
+                                        const float* saved, void* work, void* dx, void* dw_gate, void* dw_up, int T, int H,
+                                        int I, long long lddh, long long ldx, long long ldg, long long ldu, long long lddx,
+                                        long long lddw, int kind, int fmt, cudaStream_t stream) {
+  return gicc::guarded([&] {
+    gicc::ops::gated_linear_backward(dh, x, w_gate, w_up, saved, work, dx, dw_gate, dw_up, T, H, I, lddh, ldx, ldg, ldu,
+                                     lddx, lddw, kind, fmt, 0, stream);
+  });
+}

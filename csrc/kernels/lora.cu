@@ -18,6 +18,8 @@
 // Few rows: the split-K cluster core (k_lora_split); it starts while k_lora_down still runs and
 // waits for v only before its adapter blocks.  Many rows: the CTA-pair core (k_lora_pair), whose
 // lists of adapters per 256-row tile k_lora_down writes to the work area.
+//
+// Host entry points: gicc::ops::lora_linear (C++, throws) and gicc_lora_linear (C ABI).
 #include <algorithm>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -36,6 +38,7 @@ namespace lora {
 using namespace gemm;
 
 constexpr int kMaxRank = 128;
+constexpr int kMaxRows = 65535 * split::kRows;  // grid.z of k_lora_down
 constexpr int kPairRows = 2 * BM;  // rows of a pair tile
 
 // Per 256-row tile: how many adapters, which, and the lanes that each leaves alone.
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(split::kThreads)
         sum.z += q.z;
         sum.w += q.w;
       }
-      const float sc = p.scale[a];
+      const float sc = p.scale != nullptr ? p.scale[a] : 1.0f;
       const float o[4] = {sc * sum.x, sc * sum.y, sc * sum.z, sc * sum.w};
       split::store4_16(p.v + (size_t)(t0 + row) * p.r, col, p.r, o, p.fmt, 1);
     }
@@ -536,11 +539,15 @@ void check_rows(const char* name, const void* p, long long ld, int cols) {
                              " needs 16-byte aligned rows (base and pitch) of at least " + std::to_string(cols) + " elements");
 }
 template <class K>
-void allow_smem(K kernel, uint32_t bytes, bool* done) {
+void allow_smem(K kernel, uint32_t bytes, bool* done, bool shared_sm = false) {
   int dev = 0;
   GICC_CUDA(cudaGetDevice(&dev));
   if (dev < 64 && done[dev]) return;
   GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  // Kernels meant to run beside another's CTAs: without this the SM keeps just one CTA's shared
+  // memory configured, and the other kernel waits until the SM is idle.
+  if (shared_sm)
+    GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   if (dev < 64) done[dev] = true;
 }
 constexpr int kRingKb = 104;  // k_lora_split's ring: leaves room for a k_lora_down CTA on the same SM
@@ -587,8 +594,9 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   check_rows("lora_a", lora_a, K, K);
   check_rows("lora_b", lora_b, r, r);
   check_rows("work", work, 8, 8);
-  if (y == nullptr || ldy < N || adapter == nullptr || scale == nullptr)
-    throw std::runtime_error("gicc::lora_linear: y needs rows of at least N elements; adapter and scale are needed");
+  if (y == nullptr || ldy < N || adapter == nullptr)
+    throw std::runtime_error("gicc::lora_linear: y needs rows of at least N elements, and adapter is needed");
+  if (T > kMaxRows) throw std::runtime_error("gicc::lora_linear: at most " + std::to_string(kMaxRows) + " rows");
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   if (tile == 0) tile = split::pick_tile(T, N, K, 1, kRingKb, reinterpret_cast<const void*>(k_lora_split),
@@ -632,7 +640,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
                                                           (kDownBar + 15) / 16 * 16 +
                                                           (tile != 1 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows, false>)));
   static bool done_down[64] = {false};
-  allow_smem(k_lora_down, 227 * 1024, done_down);
+  allow_smem(k_lora_down, 227 * 1024, done_down, true);
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   split::launch_clusters(k_lora_down, dim3(S, d.groups, tiles), S, split::kThreads, dsmem, false, stream,
                          make_tmap_2d(x, k16, 2, T, K, ldx, d.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B), tA, d,
@@ -659,7 +667,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
     op.lists = nullptr;
     op.sV = nullptr;
     static bool done[64] = {false};
-    allow_smem(k_lora_split, 227 * 1024, done);
+    allow_smem(k_lora_split, 227 * 1024, done, true);
     split::launch_clusters(
         k_lora_split, p.grid, p.splits, split::kThreads, p.smem, true, stream,
         make_tmap_2d(x, k16, 2, T, K, ldx, p.sh.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B),
@@ -688,3 +696,11 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
 
 }  // namespace ops
 }  // namespace gicc
+
+GICC_API int gicc_lora_linear(const void* x, const void* w, const void* lora_a, const void* lora_b, const int* adapter,
+                              const float* scale, void* y, void* work, int T, int K, int N, int L, int r, long long ldx,
+                              long long ldw, long long ldy, int fmt, cudaStream_t stream) {
+  return gicc::guarded([&] {
+    gicc::ops::lora_linear(x, w, lora_a, lora_b, adapter, scale, y, work, T, K, N, L, r, ldx, ldw, ldy, fmt, 0, stream);
+  });
+}

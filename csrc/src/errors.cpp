@@ -33,6 +33,12 @@ ErrorRecord* device_error_record() {
   const int d = current_device();
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_dev[d]) return g_dev[d];
+  // The first launch may be inside a stream capture, where an allocation needs the relaxed mode.
+  struct Relaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  } relaxed;
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, sizeof(ErrorRecord));
   if (e != cudaSuccess) throw std::runtime_error(std::string("gicc: cudaMalloc(error record): ") + cudaGetErrorString(e));
