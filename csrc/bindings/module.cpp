@@ -1,8 +1,10 @@
 // module.cpp -- pybind11/torch binding of libgicc (opengda_b200._C).
 // Tensors are validated here; the kernels themselves live in libgicc.so.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include "gicc/config.hpp"
@@ -209,6 +211,17 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
 };
 
 at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, int64_t kind) {
+  // While an autograd graph made on another stream is alive, the engine would tie the leaf's
+  // accumulation there to a captured backward pass, which breaks the capture half way through.
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
+    for (const auto* t : {&x, &w_gate, &w_up})
+      if (t->requires_grad() && t->is_leaf()) {
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : c10::nullopt;
+        TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t->get_device()).unwrap(),
+                    "gated_linear: an autograd graph of this parameter from outside the capture is still alive; free it "
+                    "first, or capture gated_linear_forward and gated_linear_backward");
+      }
   return GatedLinearFn::apply(x, w_gate, w_up, kind);
 }
 

@@ -273,6 +273,30 @@ def test_autograd_step_captured():
     check(grads[1], ref[3])
 
 
+def test_capture_beside_a_live_graph_is_refused():
+    """An autograd graph of the same parameter that is alive outside the capture: refused with a
+    reason, and everything works again once it is gone."""
+    from opengda_b200.ops.ffn import gated_linear
+    x, w, _, dh = _make(8, 64, 64, torch.bfloat16, seed=15)
+    w.requires_grad_(True)
+    live = gated_linear(x, w, w)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gated_linear(x, w, w)
+    live.backward(dh)
+    _sync()
+    r = gated_ref(x, w.detach(), w.detach(), "silu", dh)
+    check(w.grad, (r[2][0] + r[3][0], 1.01 * (r[2][1] + r[3][1]) + 2.0 ** -8 * (r[2][0] + r[3][0]).abs()))
+    del live
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grad, = torch.autograd.grad(gated_linear(x, w, w), (w,), dh)
+    g.replay()
+    _sync()
+    assert torch.equal(grad, w.grad)
+
+
 def test_side_streams_at_once():
     from opengda_b200.ops.ffn import gated_linear_backward, gated_linear_forward
     jobs = []
