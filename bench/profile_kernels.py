@@ -9,6 +9,9 @@ a few launches, a few GB on the device at most.
     python bench/profile_kernels.py sgemm 8192         # torch.matmul fp32 (cuBLAS SGEMM, tf32 off), 4 launches
     python bench/profile_kernels.py jacobi 8192 8192   # k_jacobi, 4 launches
     python bench/profile_kernels.py moe 1024           # MoE layer (n=1), 2 forwards
+    python bench/profile_kernels.py gated 4096         # k_gated_pair (h 7168, i 2048; few rows: k_gated_split), 4 calls
+    python bench/profile_kernels.py gated_bwd 4096     # k_gate_grad + k_gated_bwd, 4 calls
+    python bench/profile_kernels.py lora 2048          # k_lora_down + k_lora_pair (k 4096; few rows: k_lora_split), 4 calls
     python bench/profile_kernels.py copy 268435456     # k_copy (local HBM copy)
 
 Example capture (after the same command has exited 0 without ncu):
@@ -67,6 +70,23 @@ def main():
         x, logits = make_inputs(T, 7168, 32, 0)
         for _ in range(2):
             layer(x, logits)
+    elif case in ("gated", "gated_bwd"):
+        from opengda_b200.ops.ffn import gated_linear_backward, gated_linear_forward
+        T, H, inter = args[0] if args else 4096, 7168, 2048
+        x, w_gate, w_up, dh = (torch.randn(*s, device="cuda").mul_(H ** -0.5).to(torch.bfloat16)
+                               for s in ((T, H), (inter, H), (inter, H), (T, inter)))
+        for _ in range(4):
+            _, saved = gated_linear_forward(x, w_gate, w_up, save=case == "gated_bwd")
+            if case == "gated_bwd":
+                gated_linear_backward(dh, x, w_gate, w_up, saved)
+    elif case == "lora":
+        from opengda_b200.ops.lora import lora_linear
+        T, K, L, r = args[0] if args else 2048, 4096, 64, 16
+        x, w, a, b = (torch.randn(*s, device="cuda").mul_(K ** -0.5).to(torch.bfloat16)
+                      for s in ((T, K), (K, K), (L, r, K), (L, K, r)))
+        ids = (torch.arange(T, device="cuda") * 64 // T).to(torch.int32)
+        for _ in range(4):
+            lora_linear(x, w, a, b, ids)
     elif case == "copy":
         n = args[0] if args else 1 << 28
         a = torch.empty(n, dtype=torch.uint8, device="cuda")

@@ -23,14 +23,16 @@ struct LaneLists {
   int list[ROWS];                   // distinct adapters, ascending
   int n;
 
-  // All threads of the block (at least ROWS / 2); synchronises.  An index outside [-1, L) is
-  // reported and its row treated as having no adapter.
-  __device__ void build(const int* adapter, int t0, int T, int L, ErrorRecord* err) {
+  // By `threads` threads (whole warps, at least ROWS / 2 threads), this one number `tid` of them,
+  // which synchronise on named barrier 1.  An index outside [-1, L) is reported and its row treated
+  // as having no adapter.
+  __device__ void build(const int* adapter, int t0, int T, int L, ErrorRecord* err, int tid, int threads) {
+    auto sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
     const int words = (L + 31) / 32;
     int mine[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int i = threadIdx.x + k * blockDim.x, t = t0 + i;
+      const int i = tid + k * threads, t = t0 + i;
       mine[k] = -1;
       if (i < ROWS && t < T) {
         const int a = adapter[t];
@@ -38,16 +40,16 @@ struct LaneLists {
         else if (a != -1) report_error(err, GICC_ERANGE, W_ADAPTER, -1, -1, (unsigned)a, (unsigned)L);
       }
     }
-    for (int w = threadIdx.x; w < words; w += blockDim.x) used[w] = 0;
+    for (int w = tid; w < words; w += threads) used[w] = 0;
     if (MASKS)
-      for (int i = threadIdx.x; i < ROWS * (ROWS / 32); i += blockDim.x) skip[0][i] = ~0u;
-    __syncthreads();
+      for (int i = tid; i < ROWS * (ROWS / 32); i += threads) skip[0][i] = ~0u;
+    sync();
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (mine[k] >= 0) atomicOr(&used[mine[k] >> 5], 1u << (mine[k] & 31));
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const int lane = threadIdx.x;
+    sync();
+    if (tid < 32) {
+      const int lane = tid;
       int run = 0;
       for (int w0 = 0; w0 < words; w0 += 32) {
         uint32_t b = w0 + lane < words ? used[w0 + lane] : 0u;
@@ -65,14 +67,14 @@ struct LaneLists {
       }
       if (lane == 0) n = run;
     }
-    __syncthreads();
+    sync();
     if (MASKS) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int i = threadIdx.x + k * blockDim.x;
+        const int i = tid + k * threads;
         if (mine[k] >= 0) atomicAnd(&skip[slot(mine[k])][i >> 5], ~(1u << (i & 31)));
       }
-      __syncthreads();
+      sync();
     }
   }
   // a's place in the list, for an adapter that some row uses

@@ -27,7 +27,7 @@ constexpr int kThreads = 192;
 constexpr int kMaxSplit = 8;            // portable cluster size
 constexpr int kMaxCols = 256;           // columns of all weights per tile (the MMA's N)
 constexpr int kMaxStages = 12;
-constexpr uint32_t kBarBytes = (2 * kMaxStages + 3) * 8 + 8;
+constexpr uint32_t kBarBytes = (2 * kMaxStages + 4) * 8 + 8;  // barriers, TMEM address, abort flag
 
 struct Shape {
   int T, N, K;   // rows of X, rows of each W, depth
@@ -80,11 +80,13 @@ __device__ __forceinline__ void store4_16(uint16_t* row, int col, int N, const f
 }
 
 // Op: kAccs (weights multiplied side by side) and
-//   prepare(smem_extra, t0, ...)   by all threads before the pipeline starts
+//   start(smem_extra)              by all threads before the pipeline starts
+//   kExtra                         whether there are further k-blocks after the weights'; then
+//   prepare(t0, tid)               by the 128 threads of warps 2..5, beside the pipeline
 //   loads(kb, t0, n0, x, w, bar)   the loads of k-block kb (x_bytes + w_bytes in all)
 //   idesc(n), x_desc(addr, k), w_desc(addr, k)  the MMA descriptors of k-step k of a k-block
 //   depth()                        k-blocks
-//   extra_blocks(c, S, e0, e1)     this CTA's further k-blocks after the weights'
+//   extra_blocks(c, S, e0, e1)     this CTA's further k-blocks, once prepare() is done
 //   extra_shared(t0, bar)          by the producer before the first of them: waits for what they
 //                                  need and loads what all share (arrives on bar with its bytes)
 //   extra_loads(e, n0, w, bar)     loads of one (w_bytes)
@@ -96,7 +98,9 @@ struct PlainOp {
   int type;                 // 0 = f16, 1 = bf16
   const CUtensorMap* tmX;   // set by the kernel
   const CUtensorMap* tmW;
-  __device__ void prepare(uint8_t*, int, ErrorRecord*) {}
+  static constexpr bool kExtra = false;
+  __device__ void start(uint8_t*) {}
+  __device__ void prepare(int, int) {}
   __device__ void prefetch_maps() const {
     ptx::prefetch_tmap(tmX);
     ptx::prefetch_tmap(tmW);
@@ -130,7 +134,8 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* drain = tfull + 1;
   uint64_t* once = drain + 1;  // what the further k-blocks share has landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(once + 1);
+  uint64_t* ready = once + 1;  // prepare() is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* part = reinterpret_cast<float*>(smem);  // after the last MMA: this CTA's partial
 
@@ -152,6 +157,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
     ptx::mbar_init(tfull, 1);
     ptx::mbar_init(drain, 1);
     ptx::mbar_init(once, 1);
+    ptx::mbar_init(ready, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     op.prefetch_maps();
@@ -160,17 +166,28 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
     ptx::tmem_alloc(tmem_slot, tcols);
     ptx::tmem_relinquish();
   }
-  op.prepare(after + kBarBytes, t0, err);
+  op.start(after + kBarBytes);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int nkb = op.depth();
   const int kb0 = (int)((long long)nkb * c / S), nk = (int)((long long)nkb * (c + 1) / S) - kb0;
-  int e0, e1;
-  op.extra_blocks(c, S, e0, e1);
-  const int blocks = nk + (e1 - e0);  // nk >= 1: the host takes S <= nkb
-  const int steps = (blocks + group - 1) / group;
+  // nk >= 1: the host takes S <= nkb.  With further blocks, the steps that hold only the weights'
+  // come before prepare() has to be done; then the rest, which it determines.
+  int e0 = 0, blocks = nk, steps = Op::kExtra ? nk / group : (nk + group - 1) / group;
+  auto all_steps = [&]() -> bool {
+    if (!ptx::mbar_wait(ready, 0, timeout_ns, abort_flag)) {
+      if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 5, 0);
+      *abort_flag = 1;
+      return false;
+    }
+    int e1;
+    op.extra_blocks(c, S, e0, e1);
+    blocks = nk + (e1 - e0);
+    steps = (blocks + group - 1) / group;
+    return true;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -178,7 +195,9 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
       uint32_t phase = 0;
       int issued = 0;
       bool shared = false;
-      for (int i = 0; i < steps; ++i) {
+      for (int i = 0;; ++i) {
+        if (Op::kExtra && i == nk / group && !all_steps()) break;
+        if (i >= steps) break;
         if (!ptx::mbar_wait(&empty[stage], phase ^ 1, timeout_ns, abort_flag)) {
           if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 0, 0);
           *abort_flag = 1;
@@ -220,7 +239,9 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
       int stage = 0;
       uint32_t phase = 0;
       int i = 0;
-      for (; i < steps; ++i) {
+      for (;; ++i) {
+        if (Op::kExtra && i == nk / group && !all_steps()) break;
+        if (i >= steps) break;
         if (!ptx::mbar_wait(&full[stage], phase, timeout_ns, abort_flag)) {
           if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 2, 0);
           *abort_flag = 1;
@@ -251,7 +272,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
           phase ^= 1;
         }
       }
-      if (i == steps) {
+      if (!*abort_flag) {
         ptx::mma_commit(tfull);
       } else if (i > 0) {  // aborted: wait for the MMAs in flight before TMEM is released
         ptx::mma_commit(drain);
@@ -262,6 +283,10 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
   } else {
     const int q = warp & 3;
     const int row = q * 32 + (int)lane;
+    if constexpr (Op::kExtra) {
+      op.prepare(t0, (int)threadIdx.x - 64);
+      if (threadIdx.x == 64) ptx::mbar_arrive(ready);
+    }
     if (!ptx::mbar_wait_long(tfull, 0, timeout_ns, abort_flag)) {
       if (!*abort_flag) report_error(err, GICC_ETIMEDOUT, W_GEMM_PIPE, -1, -1, 3, 0);
       *abort_flag = 1;

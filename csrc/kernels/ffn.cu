@@ -444,7 +444,7 @@ struct DxSplitOp : split::PlainOp {
   int H, I, bn;
   __device__ int depth() const { return 2 * ((I + BK - 1) / BK); }
   // k_gate_grad's results, from here on
-  __device__ void prepare(uint8_t*, int, ErrorRecord*) { ptx::griddep_wait(); }
+  __device__ void start(uint8_t*) { ptx::griddep_wait(); }
   __device__ uint32_t idesc(int n) const { return ptx::idesc_f16_f32(split::kRows, n, type, 0, 1); }
   __device__ uint64_t w_desc(uint32_t w, int k) const { return ptx::sdesc_mnmajor_sw128(w + k * 2048, 8192); }
   __device__ void loads(int kb, int t0, int n0, uint8_t* x, uint8_t* w, uint64_t* bar) const {
@@ -463,7 +463,7 @@ struct DwSplitOp : split::PlainOp {
   int T, H, bn, mblocks;
   __device__ int z() const { return (int)blockIdx.y / mblocks; }  // 0 dWg, 1 dWu
   __device__ int depth() const { return (T + BK - 1) / BK; }
-  __device__ void prepare(uint8_t*, int, ErrorRecord*) { ptx::griddep_wait(); }
+  __device__ void start(uint8_t*) { ptx::griddep_wait(); }
   __device__ uint32_t idesc(int n) const { return ptx::idesc_f16_f32(split::kRows, n, type, 1, 1); }
   __device__ uint64_t x_desc(uint32_t x, int k) const { return ptx::sdesc_mnmajor_sw128(x + k * 2048, 8192); }
   __device__ uint64_t w_desc(uint32_t w, int k) const { return ptx::sdesc_mnmajor_sw128(w + k * 2048, 8192); }

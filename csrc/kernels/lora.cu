@@ -21,6 +21,7 @@
 //
 // Host entry points: gicc::ops::lora_linear (C++, throws) and gicc_lora_linear (C ABI).
 #include <algorithm>
+#include <cstddef>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -104,6 +105,8 @@ __host__ __device__ constexpr uint32_t down_ring(int rp, int cols, int xrows, in
 constexpr uint32_t kDownBar = (2 * split::kMaxStages + 5) * 8 + 8;
 struct DownLists {
   LaneLists<split::kRows, false> tile;
+  float row_scale[split::kRows];     // of the row's adapter
+  signed char mine[split::kRows];    // the row's adapter is of this CTA's group
   alignas(16) LaneLists<kPairRows> pair;  // shared memory only where the pair lists are wanted
 };
 
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(split::kThreads)
   ptx::griddep_launch();
   const uint32_t tmem = *tmem_slot;
   // One CTA per tile reports indexes out of range.
-  lists.tile.build(p.adapter, t0, p.T, p.L, g == 0 && c == 0 ? err : nullptr);
+  lists.tile.build(p.adapter, t0, p.T, p.L, g == 0 && c == 0 ? err : nullptr, (int)threadIdx.x, split::kThreads);
   const int nkb = (p.K + BK - 1) / BK;
   const int kb0 = (int)((long long)nkb * c / S), nk = (int)((long long)nkb * (c + 1) / S) - kb0;
   const int n = lists.tile.n;
@@ -246,9 +249,13 @@ __global__ void __launch_bounds__(split::kThreads)
       const int a = p.adapter[t0 + row];
       if (a >= 0 && a < p.L) {
         const int s = lists.tile.slot(a);
-        if (s % p.groups == g) my = s / p.groups;
+        if (s % p.groups == g) {
+          my = s / p.groups;
+          lists.row_scale[row] = p.scale != nullptr ? p.scale[a] : 1.0f;
+        }
       }
     }
+    lists.mine[row] = my >= 0;
     float v[kMaxRank];
 #pragma unroll
     for (int i = 0; i < kMaxRank; ++i) v[i] = 0.f;
@@ -295,7 +302,7 @@ __global__ void __launch_bounds__(split::kThreads)
   if (p.lists.count != nullptr && g == 0 && c == 0 && (blockIdx.z & 1) == 0) {
     // the list of the 256-row tile that starts here, for the CTA-pair projection
     const int tile = blockIdx.z >> 1;
-    lists.pair.build(p.adapter, t0, p.T, p.L, nullptr);
+    lists.pair.build(p.adapter, t0, p.T, p.L, nullptr, (int)threadIdx.x, split::kThreads);
     const int m = lists.pair.n;  // <= min(L, 256) = cap
     for (int i = threadIdx.x; i < m; i += blockDim.x) p.lists.list[(size_t)tile * p.lists.cap + i] = lists.pair.list[i];
     for (int i = threadIdx.x; i < m * 8; i += blockDim.x)
@@ -310,8 +317,7 @@ __global__ void __launch_bounds__(split::kThreads)
     const int j1 = (int)((long long)items * (c + 1) / S);
     for (int j = (int)((long long)items * c / S) + (int)threadIdx.x; j < j1; j += split::kThreads) {
       const int row = j / g4, col = (j - row * g4) * 4;
-      const int a = p.adapter[t0 + row];
-      if (a < 0 || a >= p.L || lists.tile.slot(a) % p.groups != g) continue;
+      if (!lists.mine[row]) continue;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       const uint32_t off = base + (row * split::pitch(1, p.rp) + col) * 4;
       for (int s = 0; s < S; ++s) {
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(split::kThreads)
         sum.z += q.z;
         sum.w += q.w;
       }
-      const float sc = p.scale != nullptr ? p.scale[a] : 1.0f;
+      const float sc = lists.row_scale[row];
       const float o[4] = {sc * sum.x, sc * sum.y, sc * sum.z, sc * sum.w};
       split::store4_16(p.v + (size_t)(t0 + row) * p.r, col, p.r, o, p.fmt, 1);
     }
@@ -345,14 +351,16 @@ struct LoraSplitOp : split::PlainOp {
   uint32_t xpiece, wpiece;  // bytes of a piece of v and of B
   const CUtensorMap* tmV;  // set by the kernel
   const CUtensorMap* tmB;
-  const LaneLists<split::kRows>* lists;
+  LaneLists<split::kRows>* lists;
   __device__ int depth() const { return (K + BK - 1) / BK; }
   uint8_t* sV;  // the tile's rows of v, piece by piece, loaded once: every CTA of the grid reads them
-  __device__ void prepare(uint8_t* smem, int t0, ErrorRecord*) {
+  static constexpr bool kExtra = true;
+  __device__ void start(uint8_t* smem) {
     sV = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~uintptr_t(1023));
-    auto* l = reinterpret_cast<LaneLists<split::kRows>*>(sV + v_bytes());
-    l->build(adapter, t0, T, L, nullptr);  // k_lora_down reports indexes out of range
-    lists = l;
+    lists = reinterpret_cast<LaneLists<split::kRows>*>(sV + v_bytes());
+  }
+  __device__ void prepare(int t0, int tid) {
+    lists->build(adapter, t0, T, L, nullptr, tid, 128);  // k_lora_down reports indexes out of range
   }
   // The MMA reads 128 rows of the last piece too; its rows behind the box are the lists.
   __host__ __device__ uint32_t v_bytes() const { return pc.each * xpiece; }
@@ -638,7 +646,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   // at least more than half of an SM's: two of these CTAs on one SM would keep k_lora_split's off it
   const uint32_t dsmem = std::max<uint32_t>(kDownMin, 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) +
                                                           (kDownBar + 15) / 16 * 16 +
-                                                          (tile != 1 ? sizeof(DownLists) : sizeof(LaneLists<split::kRows, false>)));
+                                                          (tile != 1 ? sizeof(DownLists) : offsetof(DownLists, pair)));
   static bool done_down[64] = {false};
   allow_smem(k_lora_down, 227 * 1024, done_down, true);
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
