@@ -6,8 +6,8 @@ It offers the capabilities and API of GICC/OpenGDA (lwshanbd/OpenGDA), rebuilt f
 * ``opengda_b200.parallel`` -- socket bootstrap, ``Runtime`` (symmetric memory over CUDA
   VMM, NVLS multicast), ``Barrier`` (incl. continuous mode), active messages, the
   NVSHMEM-style ``init/malloc/remote_ptr`` API and a local multi-rank launcher;
-* ``opengda_b200.ops`` -- the sm_100a kernels (tcgen05 GEMM, put/get, barrier,
-  allreduce, Jacobi, MoE routing/dispatch/combine) as torch-facing functions;
+* ``opengda_b200.ops`` -- the sm_100a kernels (tcgen05 GEMM, gated and adapted projections,
+  put/get, barrier, allreduce, Jacobi, MoE routing/dispatch/combine) as torch-facing functions;
 * ``opengda_b200.models`` -- the workloads: distributed GEMM (AG->GEMM, GEMM->RS),
   the fp32 ring-stripe matmul, Jacobi with fused halo puts (per-iteration or persistent),
   the MoE expert-parallel layer, the CPU matmul;
