@@ -45,9 +45,9 @@ __host__ __device__ constexpr int pitch(int accs, int bn) { return accs * bn + 4
 // The ring (X of all stages, then W), or the partial that takes its place.  The MMA reads 128
 // rows of X whatever xrows is: the rows behind an X box are other data of the ring, and their
 // lanes are never read; the last box has 16 KB of ring behind its start.
-__host__ __device__ constexpr uint32_t ring_bytes(int accs, int bn, int xrows, int group, int stages, int rows) {
+__host__ __device__ constexpr uint32_t ring_bytes(int accs, int bn, int xrows, int group, int stages) {
   uint32_t ring = stages * group * (x_bytes(xrows) + w_bytes(accs, bn));
-  const uint32_t reach = (stages * group - 1) * x_bytes(xrows) + kRows * BK * 2, part = rows * pitch(accs, bn) * 4;
+  const uint32_t reach = (stages * group - 1) * x_bytes(xrows) + kRows * BK * 2, part = xrows * pitch(accs, bn) * 4;
   if (reach > ring) ring = reach;
   return ((ring > part ? ring : part) + 127) / 128 * 128;
 }
@@ -128,7 +128,7 @@ __device__ __forceinline__ void split_core(const Shape& sh, Op& op, ErrorRecord*
   const uint32_t xb = x_bytes(sh.xrows), wb = w_bytes(A, sh.bn);
   uint8_t* sX = smem;
   uint8_t* sW = smem + stages * group * xb;  // per k-block: bn rows of each weight
-  uint8_t* after = smem + ring_bytes(A, sh.bn, sh.xrows, group, stages, kRows);
+  uint8_t* after = smem + ring_bytes(A, sh.bn, sh.xrows, group, stages);
   uint64_t* full = reinterpret_cast<uint64_t*>(after);
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;

@@ -66,6 +66,7 @@ inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, uint32_t extra
   for (int S = 1; S <= kMaxSplit && S <= nkb; ++S) {
     const long long at_once = clusters_at_once(kernel, S);
     for (int bn = col_step; accs * bn <= kMaxCols; bn += col_step) {
+      if ((uint32_t)p.sh.xrows * pitch(accs, bn) * 4 > ring_kb * 1024) break;  // the partial takes the ring's place
       const long long clusters = (long long)((N + bn - 1) / bn) * tt;
       const long long turns = (clusters + at_once - 1) / at_once;
       const int steps = (nkb + S - 1) / S;
@@ -85,7 +86,7 @@ inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, uint32_t extra
   const uint32_t per = p.sh.group * (x_bytes(p.sh.xrows) + w_bytes(accs, p.sh.bn));
   p.sh.stages = std::max(2, std::min<int>(kMaxStages, ring_kb * 1024 / per));
   p.grid = dim3((N + p.sh.bn - 1) / p.sh.bn * p.splits, tt, 1);
-  p.smem = 1024 + ring_bytes(accs, p.sh.bn, p.sh.xrows, p.sh.group, p.sh.stages, kRows) + kBarBytes + extra_smem;
+  p.smem = 1024 + ring_bytes(accs, p.sh.bn, p.sh.xrows, p.sh.group, p.sh.stages) + kBarBytes + extra_smem;
   return p;
 }
 

@@ -92,7 +92,7 @@ struct DownArgs {
 constexpr int kDownCols = 128;  // columns of an accumulator
 // Beside a k_lora_split CTA's ring both fit an SM.
 constexpr uint32_t kDownRing = 92 * 1024;
-constexpr uint32_t kDownMin = 116 * 1024;
+constexpr uint32_t kDownMin = 227 * 512;  // with 1 KB of the system's each, two do not fit
 __host__ __device__ constexpr uint32_t down_stage(int xrows, int cols) { return split::x_bytes(xrows) + cols * BK * 2; }
 // as split::ring_bytes: the MMA reads 128 rows from the last x box on
 __host__ __device__ constexpr uint32_t down_ring(int rp, int cols, int xrows, int stages) {
@@ -558,7 +558,8 @@ void allow_smem(K kernel, uint32_t bytes, bool* done, bool shared_sm = false) {
     GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   if (dev < 64) done[dev] = true;
 }
-constexpr int kRingKb = 104;  // k_lora_split's ring: leaves room for a k_lora_down CTA on the same SM
+// k_lora_split's ring: with v and the lists it leaves room for a k_lora_down CTA on the same SM.
+int ring_kb(int T, int r) { return 104 - (std::min(split::kRows, (T + 7) / 8 * 8) * ((r + 15) / 16 * 16) * 2 + 1023) / 1024; }
 
 template <int NH>
 void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, const Pieces& pc, const TileLists& lists,
@@ -607,14 +608,14 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   if (T > kMaxRows) throw std::runtime_error("gicc::lora_linear: at most " + std::to_string(kMaxRows) + " rows");
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
-  if (tile == 0) tile = split::pick_tile(T, N, K, 1, kRingKb, reinterpret_cast<const void*>(k_lora_split),
-                                         10.0 + (double)T * K * 2 / 4.5e6);
+  const int nkb = (K + BK - 1) / BK;
+  if (tile == 0) tile = split::pick_tile(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split),
+                                         6.0 + 0.15 * nkb + (double)T * K * 2 / 9.0e6);  // k_lora_down in front
 
   const Work lay = work_layout(T, L, r);
   uint8_t* base = static_cast<uint8_t*>(work);
   const int sms = num_sms();
   const int tiles = (T + split::kRows - 1) / split::kRows;
-  const int nkb = (K + BK - 1) / BK;
   DownArgs d;
   d.adapter = adapter;
   d.scale = scale;
@@ -656,7 +657,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
 
   const Pieces pc = pieces(r);
   if (tile == 1) {
-    split::Plan p = split::plan(T, N, K, 1, kRingKb, 0, reinterpret_cast<const void*>(k_lora_split));
+    split::Plan p = split::plan(T, N, K, 1, ring_kb(T, r), 0, reinterpret_cast<const void*>(k_lora_split));
     p.smem += LoraSplitOp::extra_smem(pc, p.sh.xrows);
     LoraSplitOp op;
     op.adapter = adapter;
