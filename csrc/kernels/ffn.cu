@@ -591,7 +591,7 @@ BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
   // the pairs; at the end the last tiles, or the deepest alone
   auto pair_us = [&](int nh, bool x, bool w) {
     if (!x && !w) return 0.0;
-    const double nn = std::ceil((double)H / (nh * pair::BN2));
+    const double nn = std::ceil(H / 32.0) * 32 / (nh * pair::BN2);  // the last column block costs its columns
     const double nx = x ? std::ceil(T / 256.0) * nn : 0, nw = w ? 2 * std::ceil(I / 256.0) * nn : 0;
     const double busy = std::min(1.0, (nx + nw) / pairs), step = nh == 2 ? 0.60 + 0.14 * busy : 0.33 + 0.07 * busy;
     const double cx = step * kx + 2.5 * nh, cw = step * kw + 2.5 * nh;
@@ -603,7 +603,8 @@ BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
   for (int nh = 2; nh >= 1; --nh)
     for (int xs = 0; xs <= (need_x ? 1 : 0); ++xs)
       for (int ws = 0; ws <= (need_w ? 1 : 0); ++ws) {
-        const double c = pair_us(nh, need_x && !xs, need_w && !ws) + (xs ? best.px.us + 2 : 0) + (ws ? best.pw.us + 2 : 0);
+        const double c = pair_us(nh, need_x && !xs, need_w && !ws) + (xs ? 1.25 * best.px.us : 0) +
+                         (ws ? 1.25 * best.pw.us : 0);  // measured to estimated, with the launch: 1.1 to 1.4
         if (cost < 0 || c < cost) {
           cost = c;
           best.x_split = xs;

@@ -609,8 +609,9 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   const int nkb = (K + BK - 1) / BK;
-  if (tile == 0) tile = split::pick_tile(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split),
-                                         6.0 + 0.15 * nkb + (double)T * K * 2 / 9.0e6);  // k_lora_down in front
+  if (tile == 0)  // the pairs have k_lora_down in front of them
+    tile = split::pick_tile(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split),
+                            6.0 + 0.15 * nkb + (double)T * K * 2 / 9.0e6);
 
   const Work lay = work_layout(T, L, r);
   uint8_t* base = static_cast<uint8_t*>(work);
@@ -644,7 +645,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   d.groups = std::max(1, std::min(most, split::clusters_at_once(reinterpret_cast<const void*>(k_lora_down), S) / tiles));
   d.cap = std::max(1, std::min(kDownCols / d.rp, (most + d.groups - 1) / d.groups));
   d.stages = std::max(2, std::min<int>(split::kMaxStages, ring / down_stage(d.xrows, d.cap * d.rp)));
-  // at least more than half of an SM's: two of these CTAs on one SM would keep k_lora_split's off it
+  // More than half of an SM's at least: two of these CTAs on one SM would keep k_lora_split's off it.
   const uint32_t dsmem = std::max<uint32_t>(kDownMin, 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) +
                                                           (kDownBar + 15) / 16 * 16 +
                                                           (tile != 1 ? sizeof(DownLists) : offsetof(DownLists, pair)));
