@@ -53,6 +53,9 @@ __device__ __forceinline__ size_t saved_at(int t, int i, int I) {
 }
 
 // ---- forward on CTA pairs ------------------------------------------------------------------
+// Bound by the tensor pipe: 8192 x 8192 -> 8192 in 1410 us (1560 TFLOP/s), 4096 x 7168 -> 2048 in
+// 165 us (1457: 128 tiles of 256 x 256 columns of h on 74 pairs).  NH = 1 halves the tile where that
+// fills the pairs better (1001 x 2056 -> 5461: 60 us against 66).
 struct GatedMaps {
   CUtensorMap x, g, u, h;
 };
@@ -142,6 +145,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::k
 }
 
 // ---- forward for few rows ------------------------------------------------------------------
+// Bound by the weights' stream from HBM: 1 x 7168 -> 2048 (58.7 MB) in 15.7 us where a plain
+// reduction over the same bytes takes 15.5, against 76 and 46 us on the pairs; 37 x 4096 -> 8200
+// (134 MB) in 27 us (26.1).  Both weights' columns go through one MMA: with few columns an MMA
+// costs its issue (0.45 us a k-block with two, 0.22 with one).
 struct GatedSplitOp : split::PlainOp {
   static constexpr int kAccs = 2;
   const CUtensorMap* tmU;  // set by the kernel
@@ -183,7 +190,7 @@ __global__ void __launch_bounds__(split::kThreads, 1)
 // two, ahead of the arithmetic, and dh one tile ahead into registers; dh, dg and du pass through
 // shared memory so that their global accesses are whole 256-byte row pieces.  Bound by its 14
 // bytes per element (saved 8, dh 2, dg and du 4).  The first block also sets the tile counter of
-// k_gated_bwd.
+// k_gated_bwd.  8192 x 8192: 132 us (7.1 TB/s; without the ring 197); 4096 x 2048: 18 us.
 constexpr int kGradCols = 128;
 constexpr int kGradPitch = kGradCols + 8;  // 16-bit words: 16-byte accesses of 8 rows on 32 banks
 constexpr uint32_t kGradPlane = 32 * kGradCols * 4;
@@ -339,7 +346,9 @@ struct BwdMaps {
 };
 
 // The backward products' tiles on CTA pairs.  TileInfo::aux: 0 dx, 1 dWg, 2 dWu.  Tiles are taken
-// in order from a counter: the products' depths differ, and the deeper comes first.
+// in order from a counter: the products' depths differ, and the deeper comes first.  Bound by the
+// tensor pipe: 8192 rows, 8192 x 8192 in 2694 us (1632 TFLOP/s), 4096 rows, 7168 x 2048 in 326 us
+// (1476), where a fixed order takes as long and one of unequal depths up to a deepest tile longer.
 template <int NH>
 struct BwdSched {
   static constexpr int kCommWarps = 0;
@@ -436,7 +445,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::k
 }
 
 // The same products on the split-K clusters: dx of few rows (over both weights' rows), or small
-// weight gradients over many rows.
+// weight gradients over many rows.  Bound by the weights' stream: dx of 16 rows, 7168 x 2048 in 15 us
+// (pairs 31); by one round of few deep tiles: dW of 8192 rows, 512 x 512 in 22 us (pairs 54).
 struct DxSplitOp : split::PlainOp {
   static constexpr int kAccs = 1;
   uint16_t* dx;
