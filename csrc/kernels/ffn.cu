@@ -348,7 +348,7 @@ struct BwdMaps {
 // The backward products' tiles on CTA pairs.  TileInfo::aux: 0 dx, 1 dWg, 2 dWu.  Tiles are taken
 // in order from a counter: the products' depths differ, and the deeper comes first.  Bound by the
 // tensor pipe: 8192 rows, 8192 x 8192 in 2694 us (1632 TFLOP/s), 4096 rows, 7168 x 2048 in 326 us
-// (1476), where a fixed order takes as long and one of unequal depths up to a deepest tile longer.
+// (1476); 1001 rows, 2056 x 5461 on 256 x 512 tiles in 121 us, 158 in a fixed order.
 template <int NH>
 struct BwdSched {
   static constexpr int kCommWarps = 0;
@@ -545,7 +545,7 @@ void launch_gated_pair(const GatedMaps& m, const GatedEpi& e, int T, int I, int 
 
 template <int NH>
 void launch_gated_bwd(const BwdMaps& m, int T, int H, int I, bool need_x, bool need_w, int fmt, unsigned int* counter,
-                      cudaStream_t stream) {
+                      uint64_t timeout_ns, cudaStream_t stream) {
   using Cf = pair::PairCfg<NH>;
   BwdSched<NH> s;
   s.counter = counter;
@@ -572,7 +572,7 @@ void launch_gated_bwd(const BwdMaps& m, int T, int H, int I, bool need_x, bool n
   allow_smem(k_gated_bwd<NH>, Cf::kSmemBytesSwizzled, done);
   const int grid = 2 * std::min(s.num_tiles(), num_sms() / 2);
   split::launch_dependent(k_gated_bwd<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
-                          device_error_record(), default_timeout_ns());
+                          device_error_record(), timeout_ns);
 }
 
 // Where the backward products run: dx and the weight gradients each on CTA pairs (together, in
@@ -726,6 +726,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     check_rows(who, "dw_up", dw_up, lddw, H);
   }
   const int Ip = grad_pitch(I);
+  const uint64_t timeout_ns = default_timeout_ns();  // reads the environment: once a call
   const BwdPlan plan = plan_bwd(T, H, I, dx != nullptr, dw_gate != nullptr, tile);
   uint16_t* dgu = static_cast<uint16_t*>(work);
   unsigned int* counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(work) + grad_counter_at(T, I));
@@ -735,7 +736,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   allow_smem(k_gate_grad, kGradSmem, grad_done);
   k_gate_grad<<<ggrid, 256, kGradSmem, stream>>>(static_cast<const uint16_t*>(dh), lddh, saved, dgu, T, I, Ip, kind, fmt,
                                                  vec16(dh, lddh) ? 1 : 0, counter, (unsigned)(num_sms() / 2),
-                                                 device_error_record(), default_timeout_ns());
+                                                 device_error_record(), timeout_ns);
   GICC_CUDA(cudaGetLastError());
 
   BwdMaps m;
@@ -752,8 +753,8 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
                            : m.d_rows;
   const bool pair_x = dx != nullptr && !plan.x_split, pair_w = dw_gate != nullptr && !plan.w_split;
   if (pair_x || pair_w) {
-    if (plan.nh == 2) launch_gated_bwd<2>(m, T, H, I, pair_x, pair_w, fmt, counter, stream);
-    else launch_gated_bwd<1>(m, T, H, I, pair_x, pair_w, fmt, counter, stream);
+    if (plan.nh == 2) launch_gated_bwd<2>(m, T, H, I, pair_x, pair_w, fmt, counter, timeout_ns, stream);
+    else launch_gated_bwd<1>(m, T, H, I, pair_x, pair_w, fmt, counter, timeout_ns, stream);
   }
   if (plan.x_split) {
     DxSplitOp op;
@@ -767,7 +768,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     static bool done[64] = {false};
     allow_smem(k_gated_dx_split, kSmemMax, done);
     split::launch_clusters(k_gated_dx_split, plan.px.grid, plan.px.splits, split::kThreads, plan.px.smem, true, stream, m,
-                           plan.px.sh, op, device_error_record(), default_timeout_ns());
+                           plan.px.sh, op, device_error_record(), timeout_ns);
   }
   if (plan.w_split) {
     DwSplitOp op;
@@ -783,7 +784,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     static bool done[64] = {false};
     allow_smem(k_gated_dw_split, kSmemMax, done);
     split::launch_clusters(k_gated_dw_split, plan.pw.grid, plan.pw.splits, split::kThreads, plan.pw.smem, true, stream, m,
-                           plan.pw.sh, op, device_error_record(), default_timeout_ns());
+                           plan.pw.sh, op, device_error_record(), timeout_ns);
   }
 }
 

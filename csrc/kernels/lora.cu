@@ -570,7 +570,7 @@ int ring_kb(int T, int r) { return 104 - (std::min(split::kRows, (T + 7) / 8 * 8
 
 template <int NH>
 void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, const Pieces& pc, const TileLists& lists,
-                 cudaStream_t stream) {
+                 uint64_t timeout_ns, cudaStream_t stream) {
   using Cf = pair::PairCfg<NH>;
   LoraSched<NH> s;
   s.T = T;
@@ -587,7 +587,7 @@ void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, cons
   allow_smem(k_lora_pair<NH>, Cf::kSmemBytesSwizzled, done);
   const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
   split::launch_dependent(k_lora_pair<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
-                          device_error_record(), default_timeout_ns());
+                          device_error_record(), timeout_ns);
 }
 }  // namespace
 }  // namespace lora
@@ -621,6 +621,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
                             6.0 + 0.15 * nkb + (double)T * K * 2 / 9.0e6);
 
   const Work lay = work_layout(T, L, r);
+  const uint64_t timeout_ns = default_timeout_ns();  // reads the environment: once a call
   uint8_t* base = static_cast<uint8_t*>(work);
   const int sms = num_sms();
   const int tiles = (T + split::kRows - 1) / split::kRows;
@@ -661,7 +662,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   split::launch_clusters(k_lora_down, dim3(S, d.groups, tiles), S, split::kThreads, dsmem, false, stream,
                          make_tmap_2d(x, k16, 2, T, K, ldx, d.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B), tA, d,
-                         device_error_record(), default_timeout_ns());
+                         device_error_record(), timeout_ns);
 
   const Pieces pc = pieces(r);
   if (tile == 1) {
@@ -691,7 +692,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
         make_tmap_2d(w, k16, 2, N, K, ldw, p.sh.bn, BK, CU_TENSOR_MAP_SWIZZLE_128B),
         make_tmap_2d(d.v, k16, 2, T, r, r, p.sh.xrows, pc.w, piece_swizzle(pc)),
         make_tmap_3d(lora_b, k16, 2, L, N, r, r, (uint64_t)N * r, p.sh.bn, pc.w, piece_swizzle(pc)), p.sh, op,
-        device_error_record(), default_timeout_ns());
+        device_error_record(), timeout_ns);
     return;
   }
   LoraMaps m;
@@ -707,8 +708,8 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   e.fmt = fmt;
   e.vec = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ldy % 8 == 0;
   m.y = e.vec ? make_tmap_2d(y, k16, 2, T, N, ldy, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : m.x;
-  if (tile == 2) launch_pair<2>(m, e, T, N, K, pc, d.lists, stream);
-  else launch_pair<1>(m, e, T, N, K, pc, d.lists, stream);
+  if (tile == 2) launch_pair<2>(m, e, T, N, K, pc, d.lists, timeout_ns, stream);
+  else launch_pair<1>(m, e, T, N, K, pc, d.lists, timeout_ns, stream);
 }
 
 }  // namespace ops
