@@ -49,8 +49,8 @@ GICC_EXPORT void gemm_tile_done_selftest(const void* A, const void* B, int M, in
 // ---- gated projection (ffn.cu) --------------------------------------------------------------
 // h = act(x Wg^T) * (x Wu^T): x [T, H], Wg and Wu [I, H], h [T, I], row-major, all f16 (fmt 0)
 // or all bf16 (fmt 1), f32 accumulation, one rounding.  H % 8 == 0 and 16-byte aligned rows of
-// x, Wg and Wu; I is free.  saved (gated_saved_floats(T, I) floats, or null) keeps g and u for
-// the backward pass.  tile: 0 by shape, 1 split-K clusters, 2 / 3 CTA pairs with 256 x 512 / 256 x 256 tiles.
+// x, Wg and Wu; I is free.  saved (gated_saved_floats(T, I) floats, 16-byte aligned, or null)
+// keeps g and u for the backward pass.  tile: 0 by shape, 1 split-K clusters, 2 / 3 CTA pairs with 256 x 512 / 256 x 256 tiles.
 enum Activation : int { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_COUNT = 3 };
 GICC_EXPORT size_t gated_saved_floats(int T, int I);
 GICC_EXPORT void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I,

@@ -629,6 +629,10 @@ void check_16(const char* who, int fmt, int kind) {
   if (fmt < 0 || fmt > 1) throw std::runtime_error(std::string(who) + ": fmt must be 0 (f16) or 1 (bf16)");
   if (kind < 0 || kind >= ops::ACT_COUNT) throw std::runtime_error(std::string(who) + ": unknown activation");
 }
+// saved is written with 16-byte stores and read by bulk copies.
+void check_saved(const char* who, const float* saved) {
+  if (reinterpret_cast<uintptr_t>(saved) & 15) throw std::runtime_error(std::string(who) + ": saved must be 16-byte aligned");
+}
 void check_rows(const char* who, const char* name, const void* p, long long ld, int cols) {
   if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15) || ld % 8 || ld < cols)
     throw std::runtime_error(std::string(who) + ": " + name + " needs 16-byte aligned rows (base and pitch) of at least " +
@@ -658,6 +662,7 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   check_rows(who, "w_gate", w_gate, ldg, H);
   check_rows(who, "w_up", w_up, ldu, H);
   if (h == nullptr || ldh < I) throw std::runtime_error("gicc::gated_linear: h needs rows of at least I elements");
+  check_saved(who, saved);
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::gated_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   if (tile == 0) tile = split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
@@ -715,6 +720,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   check_rows(who, "w_up", w_up, ldu, H);
   if (dh == nullptr || lddh < I || saved == nullptr || work == nullptr || (reinterpret_cast<uintptr_t>(work) & 15))
     throw std::runtime_error("gicc::gated_linear_backward: dh, saved and a 16-byte aligned work area are needed");
+  check_saved(who, saved);
   if ((dw_gate == nullptr) != (dw_up == nullptr))
     throw std::runtime_error("gicc::gated_linear_backward: both weight gradients or none");
   if (tile < 0 || tile > 3)
