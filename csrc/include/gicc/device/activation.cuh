@@ -59,7 +59,8 @@ __device__ __forceinline__ float value_grad(float g, int kind, float* d) {
     return g * phi;
   }
   const float s = logistic(2.0f * kGeluK * g * (1.0f + kGeluC * g * g));
-  *d = s + g * 2.0f * s * (1.0f - s) * kGeluK * (1.0f + 3.0f * kGeluC * g * g);
+  // s (1 - s) first, and g^2 bounded: it is 0 long before they overflow
+  *d = s + 2.0f * s * (1.0f - s) * g * kGeluK * (1.0f + 3.0f * kGeluC * fminf(g * g, 1e30f));
   return g * s;
 }
 

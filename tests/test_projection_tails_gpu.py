@@ -8,8 +8,9 @@ from projection_ref import act_ref, half_step
 
 pytestmark = pytest.mark.gpu
 
-# Gates whose activation is still a normal bf16 number (2^-126 = 1.2e-38).
-RANGE = {"silu": 88.5, "gelu": 12.5, "gelu_tanh": 10.0}
+# Gates whose activation is computed: gelu's to the last normal bf16 number (1.2e-38); the logistic
+# function is 0 where its argument is below -87.3 (there |silu| < 1.1e-36).
+RANGE = {"silu": 87.0, "gelu": 12.5, "gelu_tanh": 9.9}
 
 
 def _run(gates, act, dt, tile):
@@ -66,3 +67,21 @@ def _check_tails(dt, act, tile):
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 def test_gelu_tail(dt, tile):
     _check_tails(dt, "gelu", tile)
+
+
+@pytest.mark.parametrize("tile", [1, 2, 3])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_logistic_tails(dt, act, tile):
+    _check_tails(dt, act, tile)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_huge_gates(act):
+    """Beyond the square root of f32's largest value: the gate itself or 0, slopes 1 or 0, no NaN."""
+    gates = torch.tensor([2e19, -2e19, 1e30, -1e30, 3e38, -3e38], device="cuda").to(torch.bfloat16)
+    for tile in (1, 2, 3):
+        h, du, dg = _run(gates, act, torch.bfloat16, tile)
+        g = gates.double()
+        assert torch.equal(h, g.clamp_min(0)) and torch.equal(du, g.clamp_min(0)), (h, du)
+        assert torch.equal(dg, (g > 0).double()), dg
