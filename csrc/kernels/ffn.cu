@@ -129,9 +129,9 @@ struct GatedEpi : Out16Epi {
           ptx::st_v4(u + 128 * j, make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]));
         }
     }
-    if (kind == ops::ACT_SILU) combine<ops::ACT_SILU>(lo, hi);
-    else if (kind == ops::ACT_GELU) combine<ops::ACT_GELU>(lo, hi);
-    else combine<ops::ACT_GELU_TANH>(lo, hi);
+    if (kind == ops::ACT_GELU) combine<ops::ACT_GELU>(lo, hi);
+    else if (kind == ops::ACT_GELU_TANH) combine<ops::ACT_GELU_TANH>(lo, hi);
+    else combine<ops::ACT_SILU>(lo, hi);
   }
 };
 
