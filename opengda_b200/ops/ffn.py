@@ -55,7 +55,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu",
                  out: Optional[torch.Tensor] = None, tile: int = 0) -> torch.Tensor:
-    """``h[T, I] = act(x[T, H] @ w_gate[I, H]^T) * (x @ w_up[I, H]^T)``, differentiable.
+    """``h[T, I] = act(x[T, H] @ w_gate[I, H]^T) * (x @ w_up[I, H]^T)``, differentiable
+    once, in reverse mode (an argument with a forward-mode tangent is refused).
 
     bf16 or fp16 (all alike), f32 accumulation and activation, one rounding.  ``act``: "silu",
     "gelu" (erf) or "gelu_tanh".  H a multiple of 8 and 16-byte aligned rows (as ``ops.gemm``);

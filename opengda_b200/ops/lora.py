@@ -21,7 +21,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
 
     The indexes stay on the device: one outside [-1, L) gives its row no adapter and raises at
     the next ``ops.gemm.check_errors()``.  Inference only: an input that requires a gradient is
-    refused while gradients are enabled.  Runs on the current stream of x's device and can be
+    refused while gradients are enabled, one with a forward-mode tangent always.  Runs on the current stream of x's device and can be
     captured in a CUDA graph.  ``tile``: 0 by shape, 1 split-K clusters (few rows), 2 CTA pairs."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w, lora_a, lora_b) + (() if scale is None else (scale,))):
         raise RuntimeError("lora_linear has no backward pass: call it under torch.no_grad()")

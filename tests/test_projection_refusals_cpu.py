@@ -3,6 +3,7 @@ import ctypes
 import os
 
 import pytest
+import torch
 
 P, LL, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
 
@@ -30,3 +31,41 @@ def test_unaligned_saved(lib, capfd):
         _refused(lib.gicc_gated_linear(16, 16, 16, 16, 4, 16, 8, 16, 16, 16, 8, 0, 1, off, None), capfd, what)
         _refused(lib.gicc_gated_linear_backward(16, 16, 16, 16, off, 16, 16, 16, 16, 4, 16, 8, 8, 16, 16, 16, 16, 16, 0, 1,
                                                 None), capfd, what)
+
+
+def _args():
+    """Valid but for the device: reaches the check of the device where nothing before it refuses."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    gated = {"x": z(4, 16), "w_gate": z(8, 16), "w_up": z(8, 16)}
+    lora = {"x": z(4, 16), "w": z(8, 16), "lora_a": z(1, 8, 16), "lora_b": z(1, 8, 8), "adapter": torch.zeros(4, dtype=torch.int32),
+            "scale": torch.ones(1)}
+    return gated, lora
+
+
+def test_forward_mode_tangents():
+    """A dual tensor does not require a gradient: without a check its tangent is dropped."""
+    import torch.autograd.forward_ad as fwd
+    from opengda_b200.ops.ffn import gated_linear, gated_linear_backward, gated_linear_forward
+    from opengda_b200.ops.lora import lora_linear
+    gated, lora = _args()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for name in gated:
+            for grads in (False, True):
+                args = {k: t.clone().requires_grad_(grads and k != name) for k, t in gated.items()}
+                args[name] = dual(args[name])
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    gated_linear(**args)
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                gated_linear_forward(**dict(gated, **{name: dual(gated[name])}))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            gated_linear(**gated, out=dual(torch.zeros(4, 8, dtype=torch.bfloat16)))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            gated_linear_backward(dual(torch.zeros(4, 8, dtype=torch.bfloat16)), **gated, saved=torch.zeros(1024))
+        for name in ("x", "w", "lora_a", "lora_b", "scale"):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                lora_linear(**dict(lora, **{name: dual(lora[name])}))
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):  # a dual level alone refuses nothing
+            gated_linear(**gated)
+        with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            lora_linear(**lora)
