@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "gicc/config.hpp"
@@ -121,16 +122,18 @@ at::Tensor out_or_empty(const c10::optional<at::Tensor>& out, int64_t rows, int6
   return *out;
 }
 
-// A dual tensor does not require a gradient and has a valid pointer: its tangent would be lost
-// without a word.
-void check_no_tangent(const char* who, std::initializer_list<at::Tensor> tensors) {
+// Callers that would lose the launch or a derivative without a word.  torch.jit.trace records the
+// allocation of the output and not what fills it.  A dual tensor does not require a gradient and has a
+// valid pointer: its tangent would be dropped.
+void check_caller(const char* who, std::initializer_list<at::Tensor> tensors) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), who, " cannot be traced: torch.jit.trace would record an empty result");
   for (const auto& t : tensors)
     TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, " has no forward-mode derivative: an argument carries a tangent");
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_linear(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up,
                                                 int64_t kind, bool save, c10::optional<at::Tensor> out, int64_t tile) {
-  check_no_tangent("gated_linear", {x, w_gate, w_up, out.value_or(at::Tensor())});
+  check_caller("gated_linear", {x, w_gate, w_up, out.value_or(at::Tensor())});
   const int fmt = fmt_of(x, "x");
   check_rows(x, "x", x);
   check_rows(w_gate, "w_gate", x);
@@ -154,7 +157,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::T
                                                                      const at::Tensor& w_gate, const at::Tensor& w_up,
                                                                      const at::Tensor& saved, int64_t kind, bool need_dx,
                                                                      bool need_dw, int64_t tile) {
-  check_no_tangent("gated_linear_backward", {dh, x, w_gate, w_up, saved});
+  check_caller("gated_linear_backward", {dh, x, w_gate, w_up, saved});
   const int fmt = fmt_of(x, "x");
   check_rows(x, "x", x);
   check_rows(dh, "dh", x);
@@ -220,7 +223,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
 };
 
 at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, int64_t kind) {
-  check_no_tangent("gated_linear", {x, w_gate, w_up});
+  check_caller("gated_linear", {x, w_gate, w_up});
   // While an autograd graph made on another stream is alive, the engine would tie the leaf's
   // accumulation there to a captured backward pass, which breaks the capture half way through.
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
@@ -238,7 +241,7 @@ at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& w_gate, 
 at::Tensor lora_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& lora_a, const at::Tensor& lora_b,
                        const at::Tensor& adapter, const c10::optional<at::Tensor>& scale, c10::optional<at::Tensor> out,
                        int64_t tile) {
-  check_no_tangent("lora_linear", {x, w, lora_a, lora_b, scale.value_or(at::Tensor()), out.value_or(at::Tensor())});
+  check_caller("lora_linear", {x, w, lora_a, lora_b, scale.value_or(at::Tensor()), out.value_or(at::Tensor())});
   const int fmt = fmt_of(x, "x");
   check_rows(x, "x", x);
   check_rows(w, "w", x);

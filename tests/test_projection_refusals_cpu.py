@@ -69,3 +69,19 @@ def test_forward_mode_tangents():
             gated_linear(**gated)
         with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
             lora_linear(**lora)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing():
+    """A trace holds the output's allocation and not the launch: what it returns would be whatever the
+    memory held."""
+    from opengda_b200.ops.ffn import gated_linear, gated_linear_backward, gated_linear_forward
+    from opengda_b200.ops.lora import lora_linear
+    gated, lora = _args()
+    dh, saved = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(1024)
+    for f in (lambda x: gated_linear(**dict(gated, x=x)), lambda x: gated_linear_forward(**dict(gated, x=x))[0],
+              lambda x: gated_linear(x, gated["w_gate"].requires_grad_(True), gated["w_up"]),
+              lambda x: gated_linear_backward(dh, **dict(gated, x=x), saved=saved)[0], lambda x: lora_linear(**dict(lora, x=x))):
+        gated["w_gate"].requires_grad_(False)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (gated["x"],))
