@@ -8,6 +8,9 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "gicc/config.hpp"
 #include "gicc/error.hpp"
 #include "gicc/ops.hpp"
@@ -222,19 +225,37 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
   }
 };
 
+// During a capture: refuses inputs whose autograd graph has a node made on another stream, as it is for a
+// parameter (given itself, or as the source of an input) while a graph from outside the capture is alive.  The
+// engine would run that node on its stream, which ties it to the captured backward pass and breaks the
+// capture half way through.
+void check_captured_graph(std::initializer_list<at::Tensor> inputs) {
+  using torch::autograd::Node;
+  std::vector<std::shared_ptr<Node>> roots;
+  for (const auto& t : inputs)
+    if (t.requires_grad()) {
+      auto node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+      if (node) roots.push_back(std::move(node));
+    }
+  std::vector<Node*> todo;
+  std::unordered_set<Node*> seen;
+  for (const auto& n : roots)
+    if (seen.insert(n.get()).second) todo.push_back(n.get());
+  while (!todo.empty()) {
+    Node* n = todo.back();
+    todo.pop_back();
+    const auto stream = n->stream();
+    TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(stream->device_index()).unwrap(),
+                "gated_linear: an autograd graph of this parameter from outside the capture is still alive; free it "
+                "first, detach the input, or capture gated_linear_forward and gated_linear_backward");
+    for (const auto& e : n->next_edges())
+      if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());
+  }
+}
+
 at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, int64_t kind) {
   check_caller("gated_linear", {x, w_gate, w_up});
-  // While an autograd graph made on another stream is alive, the engine would tie the leaf's
-  // accumulation there to a captured backward pass, which breaks the capture half way through.
-  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
-    for (const auto* t : {&x, &w_gate, &w_up})
-      if (t->requires_grad() && t->is_leaf()) {
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto stream = node ? node->stream() : c10::nullopt;
-        TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t->get_device()).unwrap(),
-                    "gated_linear: an autograd graph of this parameter from outside the capture is still alive; free it "
-                    "first, or capture gated_linear_forward and gated_linear_backward");
-      }
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) check_captured_graph({x, w_gate, w_up});
   return GatedLinearFn::apply(x, w_gate, w_up, kind);
 }
 
