@@ -173,19 +173,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::T
                   saved.numel() == (T > 0 ? (int64_t)gicc::ops::gated_saved_floats((int)T, (int)I) : 0),
               "saved must be what gated_linear_forward kept for these shapes");
   const c10::cuda::CUDAGuard g(x.device());
-  at::Tensor dx, dw;
+  at::Tensor dx, dwg, dwu;
   if (need_dx) dx = at::empty({T, H}, x.options());
-  if (need_dw) dw = T > 0 ? at::empty({2, I, H}, x.options()) : at::zeros({2, I, H}, x.options());
+  if (need_dw) {  // apart: one weight's gradient may be freed or overwritten while the other's lives
+    dwg = T > 0 ? at::empty({I, H}, x.options()) : at::zeros({I, H}, x.options());
+    dwu = T > 0 ? at::empty({I, H}, x.options()) : at::zeros({I, H}, x.options());
+  }
   if (T > 0 && (need_dx || need_dw)) {
     at::Tensor work = at::empty({(int64_t)gicc::ops::gated_grad_bytes((int)T, (int)I)},
                                  x.options().dtype(at::kByte));
-    uint8_t* pw = need_dw ? static_cast<uint8_t*>(dw.data_ptr()) : nullptr;
     gicc::ops::gated_linear_backward(dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), saved.data_ptr<float>(),
-                                     work.data_ptr(), need_dx ? dx.data_ptr() : nullptr, pw, need_dw ? pw + 2 * I * H : nullptr,
-                                     (int)T, (int)H, (int)I, T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0),
-                                     pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, (int)tile, cur_stream());
+                                     work.data_ptr(), need_dx ? dx.data_ptr() : nullptr, need_dw ? dwg.data_ptr() : nullptr,
+                                     need_dw ? dwu.data_ptr() : nullptr, (int)T, (int)H, (int)I,
+                                     T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0), pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, (int)tile, cur_stream());
   }
-  return {dx, need_dw ? dw.select(0, 0) : at::Tensor(), need_dw ? dw.select(0, 1) : at::Tensor()};
+  return {dx, dwg, dwu};
 }
 
 // The autograd node (C++, so that neither pass takes the interpreter's lock for its own work).

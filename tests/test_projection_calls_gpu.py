@@ -44,3 +44,25 @@ def test_capture_beside_a_live_graph_of_the_weights_source():
     _sync()
     r = gated_ref(x, w, w, "silu", dh)
     check(grad, (r[2][0] + r[3][0], 1.01 * (r[2][1] + r[3][1]) + 2.0 ** -8 * (r[2][0] + r[3][0]).abs()))
+
+
+def test_weight_gradients_do_not_share_memory():
+    """A user may free or overwrite one weight's gradient without the other's."""
+    from opengda_b200.ops.ffn import gated_linear, gated_linear_backward, gated_linear_forward
+    for T in (0, 3, 300):
+        x, wg, wu, dh = _make(T, 64, 40, torch.bfloat16)
+        _, saved = gated_linear_forward(x, wg, wu)
+        _, a, b = gated_linear_backward(dh, x, wg, wu, saved)
+        assert a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr()
+        assert a.untyped_storage().nbytes() == b.untyped_storage().nbytes() == 40 * 64 * 2
+        version = b._version
+        a.mul_(2)
+        assert b._version == version
+        ws = [w.clone().requires_grad_(True) for w in (wg, wu)]
+        gated_linear(x, *ws).backward(dh)
+        _sync()
+        assert ws[0].grad.untyped_storage().data_ptr() != ws[1].grad.untyped_storage().data_ptr()
+        if T:
+            ref = gated_ref(x, wg, wu, "silu", dh)
+            check(ws[0].grad, ref[2])
+            check(ws[1].grad, ref[3])
