@@ -185,7 +185,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(const at::T
     gicc::ops::gated_linear_backward(dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), saved.data_ptr<float>(),
                                      work.data_ptr(), need_dx ? dx.data_ptr() : nullptr, need_dw ? dwg.data_ptr() : nullptr,
                                      need_dw ? dwu.data_ptr() : nullptr, (int)T, (int)H, (int)I,
-                                     T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0), pitch_of(x), pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, (int)tile, cur_stream());
+                                     T == 1 ? std::max<int64_t>(I, dh.stride(0)) : dh.stride(0), pitch_of(x),
+                                     pitch_of(w_gate), pitch_of(w_up), H, H, (int)kind, fmt, (int)tile, cur_stream());
   }
   return {dx, dwg, dwu};
 }

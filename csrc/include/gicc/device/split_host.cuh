@@ -2,6 +2,10 @@
 #pragma once
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
+#include <initializer_list>
+#include <stdexcept>
+#include <string>
 
 #include "gicc/device/split_core.cuh"
 #include "gicc/host_util.hpp"
@@ -10,8 +14,17 @@ namespace gicc {
 namespace gemm {
 namespace split {
 
+constexpr int kMaxRowBlocks = 65535;      // grid.y
+constexpr int kMaxDim = INT32_MAX - 1023;  // rounding a size up to a tile must not overflow
+
+inline void check_dims(const char* who, std::initializer_list<int> dims) {
+  for (int d : dims)
+    if (d > kMaxDim) throw std::runtime_error(std::string(who) + ": sizes up to " + std::to_string(kMaxDim));
+}
+
 struct Plan {
   Shape sh;
+  bool fits = true;  // the launch takes so many row blocks
   int splits = 1;
   dim3 grid;
   uint32_t smem = 0;
@@ -61,6 +74,7 @@ inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, uint32_t extra
   p.sh.mblocks = (T + kRows - 1) / kRows;
   p.sh.xrows = full_rows ? kRows : std::min(kRows, (T + 7) / 8 * 8);
   const int tt = p.sh.mblocks * copies;
+  p.fits = tt <= kMaxRowBlocks;
   const int nkb = depth ? depth : (K + BK - 1) / BK;
   p.us = -1;
   for (int S = 1; S <= kMaxSplit && S <= nkb; ++S) {
@@ -104,9 +118,16 @@ inline int pick_tile(int T, int N, int K, int accs, uint32_t ring_kb, const void
     const double turns = std::ceil(tiles / pairs), busy = std::min(1.0, tiles / pairs);
     return turns * nkb * (nh == 2 ? 0.60 + 0.14 * busy : 0.33 + 0.07 * busy) + (nh == 2 ? 12.0 : 10.0) + turns + pair_extra;
   };
-  const double wide = pair_us(2), narrow = pair_us(1), split = plan(T, N, K, accs, ring_kb, 0, kernel).us;
-  if (split <= wide && split <= narrow) return 1;
+  const double wide = pair_us(2), narrow = pair_us(1);
+  const Plan split = plan(T, N, K, accs, ring_kb, 0, kernel);
+  if (split.fits && split.us <= wide && split.us <= narrow) return 1;
   return wide <= narrow ? 2 : 3;
+}
+
+inline void check_fits(const char* who, const Plan& p) {
+  if (!p.fits)
+    throw std::runtime_error(std::string(who) + ": too many rows for the split clusters (" + std::to_string(kMaxRowBlocks) +
+                             " blocks of 128)");
 }
 
 // Launch in clusters of `splits`; `overlap` lets the kernel start before the previous one of

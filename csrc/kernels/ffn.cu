@@ -587,7 +587,7 @@ BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
   const int kx = 2 * ((I + BK - 1) / BK), kw = (T + BK - 1) / BK;
   BwdPlan best;
   if (need_x && (tile == 0 || tile == 1))
-    best.px = split::plan(T, H, 2 * I, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dx_split), 64, 1, kx);
+    best.px = split::plan(T, H, I, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dx_split), 64, 1, kx);
   if (need_w && (tile == 0 || tile == 1))
     best.pw = split::plan(I, H, T, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dw_split), 64, 2, kw,
                           true);
@@ -611,8 +611,8 @@ BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
   };
   double cost = -1;
   for (int nh = 2; nh >= 1; --nh)
-    for (int xs = 0; xs <= (need_x ? 1 : 0); ++xs)
-      for (int ws = 0; ws <= (need_w ? 1 : 0); ++ws) {
+    for (int xs = 0; xs <= (need_x && best.px.fits ? 1 : 0); ++xs)
+      for (int ws = 0; ws <= (need_w && best.pw.fits ? 1 : 0); ++ws) {
         const double c = pair_us(nh, need_x && !xs, need_w && !ws) + (xs ? 1.25 * best.px.us : 0) +
                          (ws ? 1.25 * best.pw.us : 0);  // measured to estimated, with the launch: 1.1 to 1.4
         if (cost < 0 || c < cost) {
@@ -657,6 +657,7 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   const char* who = "gicc::gated_linear";
   check_16(who, fmt, kind);
   if (T <= 0 || H <= 0 || I <= 0) throw std::runtime_error("gicc::gated_linear: empty shape");
+  split::check_dims(who, {T, H, I});
   if (H % 8) throw std::runtime_error("gicc::gated_linear: H must be a multiple of 8 (16-byte TMA rows)");
   check_rows(who, "x", x, ldx, H);
   check_rows(who, "w_gate", w_gate, ldg, H);
@@ -668,6 +669,7 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   if (tile == 0) tile = split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
   if (tile == 1) {
     const split::Plan p = split::plan(T, I, H, 2, kRingKb, 0, reinterpret_cast<const void*>(k_gated_split));
+    split::check_fits(who, p);
     GatedSplitOp op;
     op.h = static_cast<uint16_t*>(h);
     op.ldh = ldh;
@@ -714,6 +716,7 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   const char* who = "gicc::gated_linear_backward";
   check_16(who, fmt, kind);
   if (T <= 0 || H <= 0 || I <= 0) throw std::runtime_error("gicc::gated_linear_backward: empty shape");
+  split::check_dims(who, {T, H, I});
   if (H % 8) throw std::runtime_error("gicc::gated_linear_backward: H must be a multiple of 8 (16-byte TMA rows)");
   check_rows(who, "x", x, ldx, H);
   check_rows(who, "w_gate", w_gate, ldg, H);
@@ -734,6 +737,8 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   const int Ip = grad_pitch(I);
   const uint64_t timeout_ns = default_timeout_ns();  // reads the environment: once a call
   const BwdPlan plan = plan_bwd(T, H, I, dx != nullptr, dw_gate != nullptr, tile);
+  if (plan.x_split) split::check_fits(who, plan.px);
+  if (plan.w_split) split::check_fits(who, plan.pw);
   uint16_t* dgu = static_cast<uint16_t*>(work);
   unsigned int* counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(work) + grad_counter_at(T, I));
   const long long gtiles = (long long)((saved_cols(I) + kGradCols - 1) / kGradCols) * ((T + 31) / 32);

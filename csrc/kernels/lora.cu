@@ -603,6 +603,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   using namespace lora;
   if (fmt < 0 || fmt > 1) throw std::runtime_error("gicc::lora_linear: fmt must be 0 (f16) or 1 (bf16)");
   if (T <= 0 || K <= 0 || N <= 0 || L <= 0 || r <= 0) throw std::runtime_error("gicc::lora_linear: empty shape");
+  split::check_dims("gicc::lora_linear", {T, K, N});
   if (K % 8 || r % 8) throw std::runtime_error("gicc::lora_linear: K and r must be multiples of 8 (16-byte TMA rows)");
   if (r > kMaxRank || L > kMaxAdapters) throw std::runtime_error("gicc::lora_linear: r <= 128 and L <= 8192");
   check_rows("x", x, ldx, K);

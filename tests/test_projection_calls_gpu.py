@@ -66,3 +66,36 @@ def test_weight_gradients_do_not_share_memory():
             ref = gated_ref(x, wg, wu, "silu", dh)
             check(ws[0].grad, ref[2])
             check(ws[1].grad, ref[3])
+
+
+def test_a_refused_size_leaves_no_error_behind():
+    """More row blocks than a grid of the split clusters takes: refused, and the next call works."""
+    from opengda_b200.ops.ffn import gated_linear
+    x = torch.zeros(65536 * 128 + 1, 8, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(1, 8, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="rows"):
+        gated_linear(x, w, w, tile=1)
+    assert not gated_linear(x, w, w).any()
+    _sync()
+
+
+def test_more_rows_than_the_split_clusters_take():
+    """By shape such a call runs on the pairs; the backward products too, where a weight has that many rows."""
+    from opengda_b200.ops.ffn import gated_linear, gated_linear_backward, gated_linear_forward
+    x = torch.zeros(65536 * 128 + 1, 8, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(1, 8, device="cuda", dtype=torch.bfloat16)
+    x[-1, :2] = 1.0
+    h = gated_linear(x, w, w)
+    _sync()
+    check(h[-1:], gated_ref(x[-1:], w, w, "silu")[0])
+    assert not h[:-1].any()
+    del h
+    rows, H = 32768 * 128 + 1, 8
+    x, wg, wu, dh = _make(2, H, rows, torch.bfloat16, seed=2)
+    h, saved = gated_linear_forward(x, wg, wu)
+    with pytest.raises(RuntimeError, match="rows"):
+        gated_linear_backward(dh, x, wg, wu, saved, tile=1)
+    got = (h, *gated_linear_backward(dh, x, wg, wu, saved))
+    _sync()
+    for t, r in zip(got, gated_ref(x, wg, wu, "silu", dh)):
+        check(t, r)

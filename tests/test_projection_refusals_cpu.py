@@ -85,3 +85,14 @@ def test_tracing():
         gated["w_gate"].requires_grad_(False)
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (gated["x"],))
+
+
+def test_sizes_next_to_the_integers_end(lib, capfd):
+    """Rounded up to a tile such a size would overflow into a negative grid."""
+    big, what = 2 ** 31 - 8, "sizes up to"
+    for T, H, n in ((big, 16, 8), (4, big, 8), (4, 16, big)):
+        _refused(lib.gicc_gated_linear(16, 16, 16, 16, T, H, n, H, H, H, n, 0, 1, None, None), capfd, what)
+        _refused(lib.gicc_gated_linear_backward(16, 16, 16, 16, 16, 16, 16, 16, 16, T, H, n, n, H, H, H, H, H, 0, 1, None), capfd,
+                 what)
+    for T, K, n in ((big, 16, 8), (4, big, 8), (4, 16, big)):
+        _refused(lib.gicc_lora_linear(16, 16, 16, 16, 16, None, 16, 16, T, K, n, 1, 8, K, K, n, 1, None), capfd, what)
