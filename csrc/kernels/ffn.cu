@@ -26,7 +26,7 @@
 // rows, small weight gradients over many) go to the split-K cluster core instead.
 //
 // Host entry points: gicc::ops::gated_linear, gated_linear_backward (C++, throw) and
-// gicc_gated_linear, gicc_gated_linear_backward (C ABI).
+// gicc_gated_linear, gicc_gated_linear_backward (C ABI, gicc/projections.h).
 #include <algorithm>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -38,6 +38,7 @@
 #include "gicc/device/split_host.cuh"
 #include "gicc/host_util.hpp"
 #include "gicc/ops.hpp"
+#include "gicc/projections.h"
 
 namespace gicc {
 namespace ffn {
@@ -802,6 +803,15 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
 }  // namespace ops
 }  // namespace gicc
 
+static_assert(GICC_ACT_SILU == gicc::ops::ACT_SILU && GICC_ACT_GELU == gicc::ops::ACT_GELU &&
+                  GICC_ACT_GELU_TANH == gicc::ops::ACT_GELU_TANH,
+              "activations");
+GICC_API size_t gicc_gated_saved_floats(int T, int I) {
+  return T > 0 && I > 0 && std::max(T, I) <= gicc::gemm::split::kMaxDim ? gicc::ops::gated_saved_floats(T, I) : 0;
+}
+GICC_API size_t gicc_gated_grad_bytes(int T, int I) {
+  return T > 0 && I > 0 && std::max(T, I) <= gicc::gemm::split::kMaxDim ? gicc::ops::gated_grad_bytes(T, I) : 0;
+}
 GICC_API int gicc_gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I,
                                long long ldx, long long ldg, long long ldu, long long ldh, int kind, int fmt, float* saved,
                                cudaStream_t stream) {

@@ -19,7 +19,8 @@
 // waits for v only before its adapter blocks.  Many rows: the CTA-pair core (k_lora_pair), whose
 // lists of adapters per 256-row tile k_lora_down writes to the work area.
 //
-// Host entry points: gicc::ops::lora_linear (C++, throws) and gicc_lora_linear (C ABI).
+// Host entry points: gicc::ops::lora_linear (C++, throws) and gicc_lora_linear (C ABI,
+// gicc/projections.h).
 #include <algorithm>
 #include <cstddef>
 #include <cuda.h>
@@ -32,6 +33,7 @@
 #include "gicc/device/split_host.cuh"
 #include "gicc/host_util.hpp"
 #include "gicc/ops.hpp"
+#include "gicc/projections.h"
 
 namespace gicc {
 namespace lora {
@@ -716,6 +718,11 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
 }  // namespace ops
 }  // namespace gicc
 
+GICC_API size_t gicc_lora_work_bytes(int T, int L, int r) {
+  const bool ok = T > 0 && T <= gicc::lora::kMaxRows && L > 0 && L <= gicc::lora::kMaxAdapters && r > 0 &&
+                  r <= gicc::lora::kMaxRank;
+  return ok ? gicc::ops::lora_work_bytes(T, L, r) : 0;
+}
 GICC_API int gicc_lora_linear(const void* x, const void* w, const void* lora_a, const void* lora_b, const int* adapter,
                               const float* scale, void* y, void* work, int T, int K, int N, int L, int r, long long ldx,
                               long long ldw, long long ldy, int fmt, cudaStream_t stream) {

@@ -96,3 +96,29 @@ def test_sizes_next_to_the_integers_end(lib, capfd):
                  what)
     for T, K, n in ((big, 16, 8), (4, big, 8), (4, 16, big)):
         _refused(lib.gicc_lora_linear(16, 16, 16, 16, 16, None, 16, 16, T, K, n, 1, 8, K, K, n, 1, None), capfd, what)
+
+
+def test_work_sizes_of_the_c_interface(lib):
+    """What a C caller has to allocate: at least the plain arrays, padded; 0 for sizes that are refused."""
+    for f, n in (("gicc_gated_saved_floats", 2), ("gicc_gated_grad_bytes", 2), ("gicc_lora_work_bytes", 3)):
+        getattr(lib, f).argtypes, getattr(lib, f).restype = [I] * n, ctypes.c_size_t
+    for T, n in ((1, 1), (5, 33), (32, 16), (61, 37), (8192, 8192), (65600, 32800)):
+        saved = lib.gicc_gated_saved_floats(T, n)
+        assert saved == 2 * ((T + 31) // 32 * 32) * ((n + 15) // 16 * 16) >= 2 * T * n
+        assert lib.gicc_gated_grad_bytes(T, n) >= 2 * T * n * 2 + 4
+        assert lib.gicc_lora_work_bytes(T, 3, 24) >= T * 24 * 2
+    for a, b in ((0, 4), (4, 0), (-1, 4), (2 ** 31 - 1, 4), (4, 2 ** 31 - 1)):
+        assert lib.gicc_gated_saved_floats(a, b) == lib.gicc_gated_grad_bytes(a, b) == 0
+    for a, b, c in ((0, 4, 8), (4, 0, 8), (4, 8193, 8), (4, 4, 136), (2 ** 31 - 1, 4, 8)):
+        assert lib.gicc_lora_work_bytes(a, b, c) == 0
+
+
+def test_c_header_is_c(tmp_path):
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "p.c"
+    src.write_text("#include <gicc/projections.h>\n"
+                   "int main(void) { return gicc_gated_saved_floats(4, GICC_ACT_GELU) == 0; }\n")
+    p = subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I" + os.path.join(root, "csrc", "include"), "-I/usr/local/cuda/include",
+                        "-fsyntax-only", str(src)], capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0, p.stderr
