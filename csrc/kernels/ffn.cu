@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(256, 2)
     ptx::bulk_load(grad_smem + stage * 2 * kGradPlane, g, bytes, &full[stage]);
     ptx::bulk_load(grad_smem + (stage * 2 + 1) * kGradPlane, g + plane, bytes, &full[stage]);
   };
-  uint16_t pre[16];
+  alignas(16) uint16_t pre[16];  // stored in 16-byte pieces
   auto load_dh = [&](long long tile) {
     const int t0 = (int)(tile / tiles_x) * 32, i0 = (int)(tile % tiles_x) * kGradCols;
     const int rows = min(32, T - t0);
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(256, 2)
     if (lane < rows && i < cols) {
       const uint4* gp = reinterpret_cast<const uint4*>(grad_smem + stage * 2 * kGradPlane) + warp * 128 + lane;
       const uint4* dp = reinterpret_cast<const uint4*>(sd + lane * kGradPitch + warp * 16);
-      uint16_t d[16];
+      alignas(16) uint16_t d[16];
       *reinterpret_cast<uint4*>(d) = dp[0];
       *reinterpret_cast<uint4*>(d + 8) = dp[1];
       uint32_t og[8], ou[8];
