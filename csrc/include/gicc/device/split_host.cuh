@@ -1,6 +1,7 @@
 // split_host.cuh -- host side of the split-K cluster core: tile and split by shape, launch.
 #pragma once
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
@@ -31,13 +32,31 @@ struct Plan {
   double us = 0;  // expected time
 };
 
-// Clusters of S CTAs of a one-per-SM kernel that the current device runs at a time (fewer than
-// SMs / S: a cluster stays within one GPC).
-inline int clusters_at_once(const void* kernel, int S) {
-  static int cache[64][kMaxSplit + 1] = {};
+// Once per device: kernel may use `bytes` of dynamic shared memory.  Host threads may get here at once.
+template <class K>
+void allow_smem(K kernel, uint32_t bytes, std::atomic<bool>* done, bool shared_sm = false) {
   int dev = 0;
   GICC_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && cache[dev][S]) return cache[dev][S];
+  if (dev < 64 && done[dev]) return;
+  GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  // Kernels meant to run beside another's CTAs: without this the SM keeps just one CTA's shared
+  // memory configured, and the other kernel waits until the SM is idle.
+  if (shared_sm)
+    GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (dev < 64) done[dev] = true;
+}
+
+// Clusters of S CTAs of a one-per-SM kernel that the current device runs at a time (fewer than
+// SMs / S: a cluster stays within one GPC).  Every kernel that asks has kThreads threads and takes
+// more than half of an SM's shared memory, so the first one's answer (at 200 KB) holds for all.
+inline int clusters_at_once(const void* kernel, int S) {
+  static std::atomic<int> cache[64][kMaxSplit + 1] = {};
+  int dev = 0;
+  GICC_CUDA(cudaGetDevice(&dev));
+  if (dev < 64) {
+    const int known = cache[dev][S];
+    if (known) return known;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S * 256);
   cfg.blockDim = dim3(kThreads);

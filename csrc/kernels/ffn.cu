@@ -513,14 +513,6 @@ bool vec16(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p)
 CUtensorMap out_map(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, const CUtensorMap& unused) {
   return vec16(p, (long long)ld) ? make_tmap_2d(p, k16, 2, rows, cols, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) : unused;
 }
-template <class K>
-void allow_smem(K kernel, uint32_t bytes, bool* done) {
-  int dev = 0;
-  GICC_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && done[dev]) return;
-  GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  if (dev < 64) done[dev] = true;
-}
 constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr int kRingKb = 200;  // the split kernel's ring
 
@@ -536,8 +528,8 @@ void launch_gated_pair(const GatedMaps& m, const GatedEpi& e, int T, int I, int 
   s.group_m = ops::gemm_tuning().pair_group_m;
   s.fmt = e.fmt;
   s.maps = nullptr;
-  static bool done[64] = {false};
-  allow_smem(k_gated_pair<NH>, Cf::kSmemBytesSwizzled, done);
+  static std::atomic<bool> done[64] = {};
+  split::allow_smem(k_gated_pair<NH>, Cf::kSmemBytesSwizzled, done);
   const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
   k_gated_pair<NH><<<grid, Cf::kThreads, Cf::kSmemBytesSwizzled, stream>>>(m, s, e, device_error_record(),
                                                                          default_timeout_ns());
@@ -569,8 +561,8 @@ void launch_gated_bwd(const BwdMaps& m, int T, int H, int I, bool need_x, bool n
   e.I = I;
   e.vec = 1;
   e.maps = nullptr;
-  static bool done[64] = {false};
-  allow_smem(k_gated_bwd<NH>, Cf::kSmemBytesSwizzled, done);
+  static std::atomic<bool> done[64] = {};
+  split::allow_smem(k_gated_bwd<NH>, Cf::kSmemBytesSwizzled, done);
   const int grid = 2 * std::min(s.num_tiles(), num_sms() / 2);
   split::launch_dependent(k_gated_bwd<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
                           device_error_record(), timeout_ns);
@@ -683,8 +675,8 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
     op.tmX = op.tmW = op.tmU = nullptr;
     op.vec = (reinterpret_cast<uintptr_t>(h) & 7) == 0 && ldh % 4 == 0;
     op.saved = saved;
-    static bool done[64] = {false};
-    allow_smem(k_gated_split, kSmemMax, done);
+    static std::atomic<bool> done[64] = {};
+    split::allow_smem(k_gated_split, kSmemMax, done);
     split::launch_clusters(k_gated_split, p.grid, p.splits, split::kThreads, p.smem, false, stream,
                            map_128b(x, T, H, ldx, p.sh.xrows), map_128b(w_gate, I, H, ldg, p.sh.bn),
                            map_128b(w_up, I, H, ldu, p.sh.bn), p.sh, op, device_error_record(), default_timeout_ns());
@@ -744,8 +736,8 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
   unsigned int* counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(work) + grad_counter_at(T, I));
   const long long gtiles = (long long)((saved_cols(I) + kGradCols - 1) / kGradCols) * ((T + 31) / 32);
   const int ggrid = (int)std::min<long long>(gtiles, 2LL * num_sms());
-  static bool grad_done[64] = {false};
-  allow_smem(k_gate_grad, kGradSmem, grad_done);
+  static std::atomic<bool> grad_done[64] = {};
+  split::allow_smem(k_gate_grad, kGradSmem, grad_done);
   k_gate_grad<<<ggrid, 256, kGradSmem, stream>>>(static_cast<const uint16_t*>(dh), lddh, saved, dgu, T, I, Ip, kind, fmt,
                                                  vec16(dh, lddh) ? 1 : 0, counter, (unsigned)(num_sms() / 2),
                                                  device_error_record(), timeout_ns);
@@ -777,8 +769,8 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     op.H = H;
     op.I = I;
     op.bn = plan.px.sh.bn;
-    static bool done[64] = {false};
-    allow_smem(k_gated_dx_split, kSmemMax, done);
+    static std::atomic<bool> done[64] = {};
+    split::allow_smem(k_gated_dx_split, kSmemMax, done);
     split::launch_clusters(k_gated_dx_split, plan.px.grid, plan.px.splits, split::kThreads, plan.px.smem, true, stream, m,
                            plan.px.sh, op, device_error_record(), timeout_ns);
   }
@@ -793,8 +785,8 @@ void gated_linear_backward(const void* dh, const void* x, const void* w_gate, co
     op.H = H;
     op.bn = plan.pw.sh.bn;
     op.mblocks = plan.pw.sh.mblocks;
-    static bool done[64] = {false};
-    allow_smem(k_gated_dw_split, kSmemMax, done);
+    static std::atomic<bool> done[64] = {};
+    split::allow_smem(k_gated_dw_split, kSmemMax, done);
     split::launch_clusters(k_gated_dw_split, plan.pw.grid, plan.pw.splits, split::kThreads, plan.pw.smem, true, stream, m,
                            plan.pw.sh, op, device_error_record(), timeout_ns);
   }

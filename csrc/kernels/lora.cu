@@ -555,18 +555,6 @@ void check_rows(const char* name, const void* p, long long ld, int cols) {
     throw std::runtime_error(std::string("gicc::lora_linear: ") + name +
                              " needs 16-byte aligned rows (base and pitch) of at least " + std::to_string(cols) + " elements");
 }
-template <class K>
-void allow_smem(K kernel, uint32_t bytes, bool* done, bool shared_sm = false) {
-  int dev = 0;
-  GICC_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && done[dev]) return;
-  GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  // Kernels meant to run beside another's CTAs: without this the SM keeps just one CTA's shared
-  // memory configured, and the other kernel waits until the SM is idle.
-  if (shared_sm)
-    GICC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-  if (dev < 64) done[dev] = true;
-}
 // k_lora_split's ring: with v and the lists it leaves room for a k_lora_down CTA on the same SM.
 int ring_kb(int T, int r) { return 104 - (std::min(split::kRows, (T + 7) / 8 * 8) * ((r + 15) / 16 * 16) * 2 + 1023) / 1024; }
 
@@ -585,8 +573,8 @@ void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, cons
   s.fmt = e.fmt;
   s.lists = lists;
   s.maps = nullptr;
-  static bool done[64] = {false};
-  allow_smem(k_lora_pair<NH>, Cf::kSmemBytesSwizzled, done);
+  static std::atomic<bool> done[64] = {};
+  split::allow_smem(k_lora_pair<NH>, Cf::kSmemBytesSwizzled, done);
   const int grid = 2 * std::min(s.num_m * s.num_n, num_sms() / 2);
   split::launch_dependent(k_lora_pair<NH>, dim3(grid), Cf::kThreads, Cf::kSmemBytesSwizzled, stream, m, s, e,
                           device_error_record(), timeout_ns);
@@ -660,8 +648,8 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   const uint32_t dsmem = std::max<uint32_t>(kDownMin, 1024 + down_ring(d.rp, d.cap * d.rp, d.xrows, d.stages) +
                                                           (kDownBar + 15) / 16 * 16 +
                                                           (tile != 1 ? sizeof(DownLists) : offsetof(DownLists, pair)));
-  static bool done_down[64] = {false};
-  allow_smem(k_lora_down, 227 * 1024, done_down, true);
+  static std::atomic<bool> done_down[64] = {};
+  split::allow_smem(k_lora_down, 227 * 1024, done_down, true);
   const CUtensorMap tA = make_tmap_3d(lora_a, k16, 2, L, r, K, K, (uint64_t)r * K, d.rp, BK, CU_TENSOR_MAP_SWIZZLE_128B);
   split::launch_clusters(k_lora_down, dim3(S, d.groups, tiles), S, split::kThreads, dsmem, false, stream,
                          make_tmap_2d(x, k16, 2, T, K, ldx, d.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B), tA, d,
@@ -687,8 +675,8 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
     op.tmX = op.tmW = op.tmV = op.tmB = nullptr;
     op.lists = nullptr;
     op.sV = nullptr;
-    static bool done[64] = {false};
-    allow_smem(k_lora_split, 227 * 1024, done, true);
+    static std::atomic<bool> done[64] = {};
+    split::allow_smem(k_lora_split, 227 * 1024, done, true);
     split::launch_clusters(
         k_lora_split, p.grid, p.splits, split::kThreads, p.smem, true, stream,
         make_tmap_2d(x, k16, 2, T, K, ldx, p.sh.xrows, BK, CU_TENSOR_MAP_SWIZZLE_128B),

@@ -68,3 +68,59 @@ def test_lora(lib, T, K, n, L, r):
     _sync()
     check(y, lora_ref(x, w, a, b, ids, scale))
     assert bool((work[nwork:] == 0x5A).all())
+
+
+def test_first_calls_from_several_threads():
+    """A process whose first calls come from several host threads at once, each on a stream of its own
+    (ctypes leaves the interpreter's lock)."""
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import threading
+import torch
+from projection_ref import check, gated_ref
+from opengda_b200 import native
+native()
+import ctypes, os
+P, LL, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+lib = ctypes.CDLL(os.path.join(%r, "opengda_b200", "lib", "libgicc.so"))
+for f in ("gicc_gated_saved_floats", "gicc_gated_grad_bytes"):
+    getattr(lib, f).argtypes, getattr(lib, f).restype = [I] * 2, ctypes.c_size_t
+lib.gicc_gated_linear.argtypes = [P, P, P, P, I, I, I, LL, LL, LL, LL, I, I, P, P]
+lib.gicc_gated_linear_backward.argtypes = [P] * 9 + [I] * 3 + [LL] * 6 + [I, I, P]
+jobs = []
+for k, (T, H, n) in enumerate([(5, 264, 130), (700, 264, 300), (33, 512, 96), (1500, 136, 64)] * 2):
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x, wg, wu, dh = ((torch.randn(*s, device="cuda", generator=g) * c).to(torch.bfloat16)
+                     for s, c in (((T, H), 1.0), ((n, H), H ** -0.5), ((n, H), H ** -0.5), ((T, n), 0.1)))
+    saved = torch.empty(lib.gicc_gated_saved_floats(T, n), device="cuda")
+    work = torch.empty(lib.gicc_gated_grad_bytes(T, n), dtype=torch.uint8, device="cuda")
+    jobs.append((torch.cuda.Stream(), T, H, n, x, wg, wu, dh, saved, work, [torch.empty_like(t) for t in (dh, x, wg, wu)]))
+torch.cuda.synchronize()
+start, rcs = threading.Barrier(len(jobs)), []
+def run(job):
+    s, T, H, n, x, wg, wu, dh, saved, work, out = job
+    p = [t.data_ptr() for t in (x, wg, wu, dh, saved, work, *out)]
+    torch.cuda.set_device(0)
+    start.wait()
+    for _ in range(3):
+        rcs.append(lib.gicc_gated_linear(p[0], p[1], p[2], p[6], T, H, n, H, H, H, n, 0, 1, p[4], s.cuda_stream))
+        rcs.append(lib.gicc_gated_linear_backward(p[3], p[0], p[1], p[2], p[4], p[5], p[7], p[8], p[9], T, H, n, n, H, H, H, H,
+                                                  H, 0, 1, s.cuda_stream))
+threads = [threading.Thread(target=run, args=(j,)) for j in jobs]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+from opengda_b200.ops.gemm import check_errors
+check_errors()
+assert len(rcs) == 6 * len(jobs) and not any(rcs), rcs
+for _, _, _, _, x, wg, wu, dh, _, _, out in jobs:
+    for t, r in zip(out, gated_ref(x, wg, wu, "silu", dh)):
+        check(t, r)
+print("done")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    root = os.path.dirname(here)
+    r = subprocess.run([sys.executable, "-c", code % (root, here, root)], capture_output=True, text=True, timeout=180)
+    assert "done" in r.stdout, r.stdout + r.stderr
