@@ -30,7 +30,7 @@ constexpr int kMaxStages = 12;
 constexpr uint32_t kBarBytes = (2 * kMaxStages + 4) * 8 + 8;  // barriers, TMEM address, abort flag
 
 struct Shape {
-  int T, N, K;   // rows of X, rows of each W, depth
+  int T;         // rows of X
   int bn;        // columns per tile and weight: a multiple of 16
   int mblocks;   // tiles of 128 rows
   int xrows;     // rows of an X box: min(128, T rounded up to 8)

@@ -23,6 +23,14 @@ inline void check_dims(const char* who, std::initializer_list<int> dims) {
     if (d > kMaxDim) throw std::runtime_error(std::string(who) + ": sizes up to " + std::to_string(kMaxDim));
 }
 
+constexpr CUtensorMapDataType k16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // 16-bit words (f16 too: TMA moves bits)
+
+inline void check_rows(const char* who, const char* name, const void* p, long long ld, int cols) {
+  if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15) || ld % 8 || ld < cols)
+    throw std::runtime_error(std::string(who) + ": " + name + " needs 16-byte aligned rows (base and pitch) of at least " +
+                             std::to_string(cols) + " elements");
+}
+
 struct Plan {
   Shape sh;
   bool fits = true;  // the launch takes so many row blocks
@@ -84,12 +92,10 @@ inline int clusters_at_once(const void* kernel, int S) {
 // col_step: what bn is a multiple of (64 for an N-major W); copies: products of this shape in the
 // launch (grid.y = copies * row blocks); depth: k-blocks, where it is not K / 64; full_rows: every X
 // box holds 128 rows (an M-major X).
-inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, uint32_t extra_smem, const void* kernel,
+inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, const void* kernel,
                  int col_step = 16, int copies = 1, int depth = 0, bool full_rows = false) {
   Plan p;
   p.sh.T = T;
-  p.sh.N = N;
-  p.sh.K = K;
   p.sh.mblocks = (T + kRows - 1) / kRows;
   p.sh.xrows = full_rows ? kRows : std::min(kRows, (T + 7) / 8 * 8);
   const int tt = p.sh.mblocks * copies;
@@ -119,7 +125,7 @@ inline Plan plan(int T, int N, int K, int accs, uint32_t ring_kb, uint32_t extra
   const uint32_t per = p.sh.group * (x_bytes(p.sh.xrows) + w_bytes(accs, p.sh.bn));
   p.sh.stages = std::max(2, std::min<int>(kMaxStages, ring_kb * 1024 / per));
   p.grid = dim3((N + p.sh.bn - 1) / p.sh.bn * p.splits, tt, 1);
-  p.smem = 1024 + ring_bytes(accs, p.sh.bn, p.sh.xrows, p.sh.group, p.sh.stages) + kBarBytes + extra_smem;
+  p.smem = 1024 + ring_bytes(accs, p.sh.bn, p.sh.xrows, p.sh.group, p.sh.stages) + kBarBytes;
   return p;
 }
 
@@ -138,7 +144,7 @@ inline int pick_tile(int T, int N, int K, int accs, uint32_t ring_kb, const void
     return turns * nkb * (nh == 2 ? 0.60 + 0.14 * busy : 0.33 + 0.07 * busy) + (nh == 2 ? 12.0 : 10.0) + turns + pair_extra;
   };
   const double wide = pair_us(2), narrow = pair_us(1);
-  const Plan split = plan(T, N, K, accs, ring_kb, 0, kernel);
+  const Plan split = plan(T, N, K, accs, ring_kb, kernel);
   if (split.fits && split.us <= wide && split.us <= narrow) return 1;
   return wide <= narrow ? 2 : 3;
 }

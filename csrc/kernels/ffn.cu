@@ -66,7 +66,7 @@ struct GatedSched {
   static constexpr int kCols = NH * pair::BN2 / 2;  // columns of h per tile
   static constexpr int kCommWarps = 0;
   static constexpr bool kOwnOperands = true;
-  int T, I, H;
+  int I, H;
   int num_m, num_n, group_m;
   int fmt;
   const GatedMaps* maps;  // set by the kernel
@@ -504,7 +504,8 @@ __global__ void __launch_bounds__(split::kThreads, 1)
 }
 
 namespace {
-constexpr CUtensorMapDataType k16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // 16-bit words (f16 too: TMA moves bits)
+using split::check_rows;
+using split::k16;
 
 CUtensorMap map_128b(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
   return make_tmap_2d(p, k16, 2, rows, cols, ld, box_rows, BK, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -520,7 +521,6 @@ template <int NH>
 void launch_gated_pair(const GatedMaps& m, const GatedEpi& e, int T, int I, int H, cudaStream_t stream) {
   using Cf = pair::PairCfg<NH>;
   GatedSched<NH> s;
-  s.T = T;
   s.I = I;
   s.H = H;
   s.num_m = (T + 2 * BM - 1) / (2 * BM);
@@ -580,9 +580,9 @@ BwdPlan plan_bwd(int T, int H, int I, bool need_x, bool need_w, int tile) {
   const int kx = 2 * ((I + BK - 1) / BK), kw = (T + BK - 1) / BK;
   BwdPlan best;
   if (need_x && (tile == 0 || tile == 1))
-    best.px = split::plan(T, H, I, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dx_split), 64, 1, kx);
+    best.px = split::plan(T, H, I, 1, kRingKb, reinterpret_cast<const void*>(k_gated_dx_split), 64, 1, kx);
   if (need_w && (tile == 0 || tile == 1))
-    best.pw = split::plan(I, H, T, 1, kRingKb, 0, reinterpret_cast<const void*>(k_gated_dw_split), 64, 2, kw,
+    best.pw = split::plan(I, H, T, 1, kRingKb, reinterpret_cast<const void*>(k_gated_dw_split), 64, 2, kw,
                           true);
   if (tile) {
     best.x_split = tile == 1 && need_x;
@@ -626,11 +626,6 @@ void check_16(const char* who, int fmt, int kind) {
 void check_saved(const char* who, const float* saved) {
   if (reinterpret_cast<uintptr_t>(saved) & 15) throw std::runtime_error(std::string(who) + ": saved must be 16-byte aligned");
 }
-void check_rows(const char* who, const char* name, const void* p, long long ld, int cols) {
-  if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15) || ld % 8 || ld < cols)
-    throw std::runtime_error(std::string(who) + ": " + name + " needs 16-byte aligned rows (base and pitch) of at least " +
-                             std::to_string(cols) + " elements");
-}
 }  // namespace
 }  // namespace ffn
 
@@ -661,7 +656,7 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
     throw std::runtime_error("gicc::gated_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   if (tile == 0) tile = split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
   if (tile == 1) {
-    const split::Plan p = split::plan(T, I, H, 2, kRingKb, 0, reinterpret_cast<const void*>(k_gated_split));
+    const split::Plan p = split::plan(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
     split::check_fits(who, p);
     GatedSplitOp op;
     op.h = static_cast<uint16_t*>(h);

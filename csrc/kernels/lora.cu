@@ -444,7 +444,7 @@ struct LoraSched {
   static constexpr bool kOwnOperands = true;
   static constexpr bool kLanes = true;
   static constexpr bool kDependent = true;
-  int T, N, K;
+  int N, K;
   Pieces pc;
   int num_m, num_n, group_m;
   int fmt;
@@ -532,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::k
 }
 
 namespace {
-constexpr CUtensorMapDataType k16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // 16-bit words (f16 too: TMA moves bits)
+using split::k16;
 
 struct Work {
   size_t v, count, list, skip, bytes;
@@ -550,11 +550,6 @@ Work work_layout(int T, int L, int r) {
   w.bytes = w.skip + up(tiles * w.cap * 32);
   return w;
 }
-void check_rows(const char* name, const void* p, long long ld, int cols) {
-  if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15) || ld % 8 || ld < cols)
-    throw std::runtime_error(std::string("gicc::lora_linear: ") + name +
-                             " needs 16-byte aligned rows (base and pitch) of at least " + std::to_string(cols) + " elements");
-}
 // k_lora_split's ring: with v and the lists it leaves room for a k_lora_down CTA on the same SM.
 int ring_kb(int T, int r) { return 104 - (std::min(split::kRows, (T + 7) / 8 * 8) * ((r + 15) / 16 * 16) * 2 + 1023) / 1024; }
 
@@ -563,7 +558,6 @@ void launch_pair(const LoraMaps& m, const Out16Epi& e, int T, int N, int K, cons
                  uint64_t timeout_ns, cudaStream_t stream) {
   using Cf = pair::PairCfg<NH>;
   LoraSched<NH> s;
-  s.T = T;
   s.N = N;
   s.K = K;
   s.pc = pc;
@@ -591,16 +585,17 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
                  long long ldy, int fmt, int tile, cudaStream_t stream) {
   NvtxRange nvtx("gicc::ops::lora_linear");
   using namespace lora;
+  const char* who = "gicc::lora_linear";
   if (fmt < 0 || fmt > 1) throw std::runtime_error("gicc::lora_linear: fmt must be 0 (f16) or 1 (bf16)");
   if (T <= 0 || K <= 0 || N <= 0 || L <= 0 || r <= 0) throw std::runtime_error("gicc::lora_linear: empty shape");
-  split::check_dims("gicc::lora_linear", {T, K, N});
+  split::check_dims(who, {T, K, N});
   if (K % 8 || r % 8) throw std::runtime_error("gicc::lora_linear: K and r must be multiples of 8 (16-byte TMA rows)");
   if (r > kMaxRank || L > kMaxAdapters) throw std::runtime_error("gicc::lora_linear: r <= 128 and L <= 8192");
-  check_rows("x", x, ldx, K);
-  check_rows("w", w, ldw, K);
-  check_rows("lora_a", lora_a, K, K);
-  check_rows("lora_b", lora_b, r, r);
-  check_rows("work", work, 8, 8);
+  split::check_rows(who, "x", x, ldx, K);
+  split::check_rows(who, "w", w, ldw, K);
+  split::check_rows(who, "lora_a", lora_a, K, K);
+  split::check_rows(who, "lora_b", lora_b, r, r);
+  split::check_rows(who, "work", work, 8, 8);
   if (y == nullptr || ldy < N || adapter == nullptr)
     throw std::runtime_error("gicc::lora_linear: y needs rows of at least N elements, and adapter is needed");
   if (T > kMaxRows) throw std::runtime_error("gicc::lora_linear: at most " + std::to_string(kMaxRows) + " rows");
@@ -657,7 +652,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
 
   const Pieces pc = pieces(r);
   if (tile == 1) {
-    split::Plan p = split::plan(T, N, K, 1, ring_kb(T, r), 0, reinterpret_cast<const void*>(k_lora_split));
+    split::Plan p = split::plan(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split));
     p.smem += LoraSplitOp::extra_smem(pc, p.sh.xrows);
     LoraSplitOp op;
     op.adapter = adapter;
