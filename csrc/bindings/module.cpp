@@ -373,6 +373,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_linear", &gated_linear, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("act") = 0,
         py::arg("save") = false, py::arg("out") = py::none(), py::arg("tile") = 0,
         "h = act(x w_gate^T) * (x w_up^T); (h, what the backward pass needs)");
+  m.def("gated_linear_tile", &gicc::ops::gated_linear_tile, py::arg("T"), py::arg("H"), py::arg("I"),
+        "the tile that gated_linear picks for these sizes on the current device");
+  m.def("lora_linear_tile", &gicc::ops::lora_linear_tile, py::arg("T"), py::arg("K"), py::arg("N"), py::arg("r"),
+        "the tile that lora_linear picks for these sizes on the current device");
   m.def("gated_linear_autograd", &gated_linear_autograd, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("act") = 0,
         "gated_linear as a node of the autograd graph");
   m.def("gated_linear_backward", &gated_linear_backward, py::arg("dh"), py::arg("x"), py::arg("w_gate"), py::arg("w_up"),

@@ -20,7 +20,7 @@ constexpr int kMaxDim = INT32_MAX - 1023;  // rounding a size up to a tile must 
 
 inline void check_dims(const char* who, std::initializer_list<int> dims) {
   for (int d : dims)
-    if (d > kMaxDim) throw std::runtime_error(std::string(who) + ": sizes up to " + std::to_string(kMaxDim));
+    if (d <= 0 || d > kMaxDim) throw std::runtime_error(std::string(who) + ": sizes from 1 to " + std::to_string(kMaxDim));
 }
 
 constexpr CUtensorMapDataType k16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;  // 16-bit words (f16 too: TMA moves bits)

@@ -51,8 +51,10 @@ GICC_EXPORT void gemm_tile_done_selftest(const void* A, const void* B, int M, in
 // or all bf16 (fmt 1), f32 accumulation, one rounding.  H % 8 == 0 and 16-byte aligned rows of
 // x, Wg and Wu; I is free.  saved (gated_saved_floats(T, I) floats, 16-byte aligned, or null)
 // keeps g and u for the backward pass.  tile: 0 by shape, 1 split-K clusters, 2 / 3 CTA pairs with 256 x 512 / 256 x 256 tiles.
+// gated_linear_tile: the tile that 0 stands for.
 enum Activation : int { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_COUNT = 3 };
 GICC_EXPORT size_t gated_saved_floats(int T, int I);
+GICC_EXPORT int gated_linear_tile(int T, int H, int I);
 GICC_EXPORT void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I,
                               long long ldx, long long ldg, long long ldu, long long ldh, int kind, int fmt, float* saved,
                               int tile, cudaStream_t stream);
@@ -69,8 +71,9 @@ GICC_EXPORT void gated_linear_backward(const void* dh, const void* x, const void
 // y[t] = W x[t] + scale[a] B[a] (A[a] x[t]), a = adapter[t] (-1: none): x [T, K], W [N, K],
 // A [L, r, K], B [L, N, r] (dense), y [T, N], all f16 (fmt 0) or all bf16 (fmt 1); adapter
 // int32 [T], scale f32 [L] or null (1).  K % 8 == 0, r % 8 == 0, r <= 128, L <= 8192.  work holds
-// lora_work_bytes(T, L, r).  tile as for gated_linear.
+// lora_work_bytes(T, L, r).  tile as for gated_linear; lora_linear_tile: the tile that 0 stands for.
 GICC_EXPORT size_t lora_work_bytes(int T, int L, int r);
+GICC_EXPORT int lora_linear_tile(int T, int K, int N, int r);
 GICC_EXPORT void lora_linear(const void* x, const void* w, const void* lora_a, const void* lora_b, const int* adapter,
                              const float* scale, void* y, void* work, int T, int K, int N, int L, int r, long long ldx,
                              long long ldw, long long ldy, int fmt, int tile, cudaStream_t stream);

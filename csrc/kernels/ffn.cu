@@ -637,6 +637,12 @@ static size_t grad_counter_at(int T, int I) { return (size_t)2 * T * grad_pitch(
 size_t gated_saved_floats(int T, int I) { return 2 * ffn::saved_plane(T, I); }
 size_t gated_grad_bytes(int T, int I) { return grad_counter_at(T, I) + 16; }
 
+int gated_linear_tile(int T, int H, int I) {
+  using namespace ffn;
+  split::check_dims("gicc::gated_linear_tile", {T, H, I});
+  return split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
+}
+
 void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, int T, int H, int I, long long ldx,
                   long long ldg, long long ldu, long long ldh, int kind, int fmt, float* saved, int tile,
                   cudaStream_t stream) {
@@ -654,7 +660,7 @@ void gated_linear(const void* x, const void* w_gate, const void* w_up, void* h, 
   check_saved(who, saved);
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::gated_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
-  if (tile == 0) tile = split::pick_tile(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
+  if (tile == 0) tile = gated_linear_tile(T, H, I);
   if (tile == 1) {
     const split::Plan p = split::plan(T, I, H, 2, kRingKb, reinterpret_cast<const void*>(k_gated_split));
     split::check_fits(who, p);

@@ -580,6 +580,13 @@ namespace ops {
 
 size_t lora_work_bytes(int T, int L, int r) { return lora::work_layout(T, L, r).bytes; }
 
+int lora_linear_tile(int T, int K, int N, int r) {
+  using namespace lora;  // the pairs have k_lora_down in front of them
+  split::check_dims("gicc::lora_linear_tile", {T, K, N, r});
+  return split::pick_tile(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split),
+                          6.0 + 0.15 * ((K + BK - 1) / BK) + (double)T * K * 2 / 9.0e6);
+}
+
 void lora_linear(const void* x, const void* w, const void* lora_a, const void* lora_b, const int* adapter,
                  const float* scale, void* y, void* work, int T, int K, int N, int L, int r, long long ldx, long long ldw,
                  long long ldy, int fmt, int tile, cudaStream_t stream) {
@@ -602,9 +609,7 @@ void lora_linear(const void* x, const void* w, const void* lora_a, const void* l
   if (tile < 0 || tile > 3)
     throw std::runtime_error("gicc::lora_linear: tile must be 0 (by shape), 1 (split), 2 (pairs, 256 x 512) or 3 (pairs, 256 x 256)");
   const int nkb = (K + BK - 1) / BK;
-  if (tile == 0)  // the pairs have k_lora_down in front of them
-    tile = split::pick_tile(T, N, K, 1, ring_kb(T, r), reinterpret_cast<const void*>(k_lora_split),
-                            6.0 + 0.15 * nkb + (double)T * K * 2 / 9.0e6);
+  if (tile == 0) tile = lora_linear_tile(T, K, N, r);
 
   const Work lay = work_layout(T, L, r);
   const uint64_t timeout_ns = default_timeout_ns();  // reads the environment: once a call

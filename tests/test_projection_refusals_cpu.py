@@ -89,7 +89,7 @@ def test_tracing():
 
 def test_sizes_next_to_the_integers_end(lib, capfd):
     """Rounded up to a tile such a size would overflow into a negative grid."""
-    big, what = 2 ** 31 - 8, "sizes up to"
+    big, what = 2 ** 31 - 8, "sizes from 1 to"
     for T, H, n in ((big, 16, 8), (4, big, 8), (4, 16, big)):
         _refused(lib.gicc_gated_linear(16, 16, 16, 16, T, H, n, H, H, H, n, 0, 1, None, None), capfd, what)
         _refused(lib.gicc_gated_linear_backward(16, 16, 16, 16, 16, 16, 16, 16, 16, T, H, n, n, H, H, H, H, H, 0, 1, None), capfd,
@@ -122,3 +122,12 @@ def test_c_header_is_c(tmp_path):
     p = subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I" + os.path.join(root, "csrc", "include"), "-I/usr/local/cuda/include",
                         "-fsyntax-only", str(src)], capture_output=True, text=True, timeout=120)
     assert p.returncode == 0, p.stderr
+
+
+def test_sizes_asked_for_their_tile():
+    from opengda_b200 import native
+    for sizes in ((0, 64, 8), (4, 0, 8), (4, 64, 0), (2 ** 31 - 8, 64, 8)):
+        with pytest.raises(RuntimeError, match="sizes from 1 to"):
+            native().gated_linear_tile(*sizes)
+        with pytest.raises(RuntimeError, match="sizes from 1 to"):
+            native().lora_linear_tile(*sizes, 8)
