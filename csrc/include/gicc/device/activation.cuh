@@ -7,7 +7,9 @@
 namespace gicc {
 namespace act {
 
-// x / (1 + e^-t).  A t far below zero makes the exponential infinite and the quotient 0.
+// 1 / (1 + e^-t).  0 where t is below -87.3: __fdividef gives 0 for a divisor beyond 2^126.  (By the
+// exponential of -|t| it would go on, but 8192 x 1024 -> 8192 took 227 to 243 us instead of 216 with it,
+// for values of silu below 1.1e-36.)
 __device__ __forceinline__ float logistic(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
 
 // Phi(g) = (1 + erf(g / sqrt 2)) / 2, and e^(-g^2/2) in *e.  The sum with erf cancels where g is far

@@ -3,7 +3,9 @@
  * All matrices are row-major with unit column stride, on the current device, all f16 (fmt 0) or all
  * bf16 (fmt 1); ld* are row pitches in elements.  x, the weights, lora_a, lora_b and the gradients
  * have 16-byte aligned rows (base and pitch); saved and work are 16-byte aligned.  Sizes are 1 or more,
- * H, K and r multiples of 8.  The calls launch on `stream`, allocate nothing and can be captured.
+ * H, K and r multiples of 8.  Outputs, saved and work overlap neither the inputs nor one another.  The
+ * calls launch on `stream`, allocate nothing but the device's error record (first call of the library)
+ * and can be captured.
  * They return 0, or -1 with the reason on stderr.
  *
  * gicc_gated_linear            h[T,I] = act(x[T,H] w_gate[I,H]^T) * (x w_up[I,H]^T).  saved: null, or

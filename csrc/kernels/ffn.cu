@@ -146,10 +146,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::PairCfg<NH>::k
 }
 
 // ---- forward for few rows ------------------------------------------------------------------
-// Bound by the weights' stream from HBM: 1 x 7168 -> 2048 (58.7 MB) in 15.7 us where a plain
-// reduction over the same bytes takes 15.5, against 76 and 46 us on the pairs; 37 x 4096 -> 8200
-// (134 MB) in 27 us (26.1).  Both weights' columns go through one MMA: with few columns an MMA
-// costs its issue (0.45 us a k-block with two, 0.22 with one).
+// Bound by the weights' stream from HBM behind 6 us of launch, first loads and the cluster's sum: 1 x
+// 7168 -> 2048 (58.7 MB) in 18.5 us a call of a CUDA graph, against 76 and 46 us on the pairs; 37 x 4096
+// -> 8200 (134 MB) in 28.5.  Both weights' columns go through one MMA: with few columns an MMA costs its
+// issue (0.45 us a k-block with two, 0.22 with one).
 struct GatedSplitOp : split::PlainOp {
   static constexpr int kAccs = 2;
   const CUtensorMap* tmU;  // set by the kernel
@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(split::kThreads, 1)
 // two, ahead of the arithmetic, and dh one tile ahead into registers; dh, dg and du pass through
 // shared memory so that their global accesses are whole 256-byte row pieces.  Bound by its 14
 // bytes per element (saved 8, dh 2, dg and du 4).  The first block also sets the tile counter of
-// k_gated_bwd.  8192 x 8192: 132 us (7.1 TB/s; without the ring 197); 4096 x 2048: 18 us.
+// k_gated_bwd.  8192 x 8192: 132 us (without the ring 197; the 671 MB read alone take 103 at 6.54 TB/s,
+// the last of the 268 MB written stay in L2); 4096 x 2048: 18 us.
 constexpr int kGradCols = 128;
 constexpr int kGradPitch = kGradCols + 8;  // 16-bit words: 16-byte accesses of 8 rows on 32 banks
 constexpr uint32_t kGradPlane = 32 * kGradCols * 4;

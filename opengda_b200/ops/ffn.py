@@ -48,7 +48,8 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
                           need_dw: bool = True, tile: int = 0) -> Tuple[Optional[torch.Tensor], ...]:
     """Gradients ``(dx, dw_gate, dw_up)`` of ``gated_linear`` from ``dh`` (row-major) and the
     forward's ``saved``; None for those not wanted.  The gradients of g and u are rounded to the
-    inputs' type once, between the activation's derivative and the products; sums are f32."""
+    inputs' type once, between the activation's derivative and the products (in fp16, scale the loss so
+    that they stay above 6e-5); sums are f32."""
     return native().gated_linear_backward(dh, x, w_gate, w_up, saved, _act(act), bool(need_dx), bool(need_dw),
                                           int(tile))
 
@@ -60,8 +61,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
 
     bf16 or fp16 (all alike), f32 accumulation and activation, one rounding.  ``act``: "silu",
     "gelu" (erf) or "gelu_tanh".  H a multiple of 8 and 16-byte aligned rows (as ``ops.gemm``);
-    T and I are free.  ``out`` and ``tile`` (0 by shape, 1 split-K clusters for few rows, 2 CTA
-    pairs) are for calls without gradients.
+    T and I are free.  ``out`` and ``tile`` (0 by shape, 1 split-K clusters for few rows, 2 and 3
+    CTA pairs with 256 x 512 and 256 x 256 tiles) are for calls without gradients.
 
     Runs on the current stream of x's device and can be captured in a CUDA graph.  To capture a
     training step, call ``gated_linear_forward`` and ``gated_linear_backward``, or make sure that
