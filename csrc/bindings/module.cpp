@@ -228,10 +228,11 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
   }
 };
 
-// During a capture: refuses inputs whose autograd graph has a node made on another stream, as it is for a
-// parameter (given itself, or as the source of an input) while a graph from outside the capture is alive.  The
-// engine would run that node on its stream, which ties it to the captured backward pass and breaks the
-// capture half way through.
+// During a capture: refuses inputs whose autograd graph has a node made on the default stream, as it is for
+// a parameter (given itself, or as the source of an input) while a graph from outside the capture is alive.
+// The engine would run that node there, and a default stream that waits for a captured one breaks the
+// capture half way through.  Nodes of other streams (a warm-up's, as in torch.cuda.make_graphed_callables) are
+// joined by the engine.
 void check_captured_graph(std::initializer_list<at::Tensor> inputs) {
   using torch::autograd::Node;
   std::vector<std::shared_ptr<Node>> roots;
@@ -248,8 +249,8 @@ void check_captured_graph(std::initializer_list<at::Tensor> inputs) {
     Node* n = todo.back();
     todo.pop_back();
     const auto stream = n->stream();
-    TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(stream->device_index()).unwrap(),
-                "gated_linear: an autograd graph of this parameter from outside the capture is still alive; free it "
+    TORCH_CHECK(!stream.has_value() || *stream != at::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                "gated_linear: an autograd graph of this parameter from the default stream is still alive; free it "
                 "first, detach the input, or capture gated_linear_forward and gated_linear_backward");
     for (const auto& e : n->next_edges())
       if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());

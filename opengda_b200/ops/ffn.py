@@ -66,8 +66,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
 
     Runs on the current stream of x's device and can be captured in a CUDA graph.  To capture a
     training step, call ``gated_linear_forward`` and ``gated_linear_backward``, or make sure that
-    no eager autograd graph of the same parameters (or of what the weights are computed from) is
-    alive: such a call is refused."""
+    no autograd graph made on the default stream of the same parameters (or of what the weights are
+    computed from) is alive: such a call is refused."""
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         if out is not None or tile:
             raise ValueError("gated_linear: out and tile are for calls without gradients")

@@ -99,3 +99,59 @@ def test_more_rows_than_the_split_clusters_take():
     _sync()
     for t, r in zip(got, gated_ref(x, wg, wu, "silu", dh)):
         check(t, r)
+
+
+def test_capture_beside_a_live_graph_of_another_side_stream():
+    """A warm-up on a stream of its own whose result is still held: the engine joins that stream."""
+    from opengda_b200.ops.ffn import gated_linear
+    x, wg, wu, dh = _make(130, 72, 96, torch.bfloat16, seed=3)
+    wg.requires_grad_(True)
+    wu.requires_grad_(True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        live = gated_linear(x, wg, wu)
+        torch.autograd.grad(live, (wg, wu), dh, retain_graph=True)
+    torch.cuda.synchronize()
+    g, acc = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grads = torch.autograd.grad(gated_linear(x, wg, wu), (wg, wu), dh)
+    wg.grad, wu.grad = torch.zeros_like(wg), torch.zeros_like(wu)
+    with torch.cuda.graph(acc):
+        wg.grad.zero_()
+        wu.grad.zero_()
+        gated_linear(x, wg, wu).backward(dh)
+    x.copy_(_make(130, 72, 96, torch.bfloat16, seed=4)[0])
+    g.replay()
+    acc.replay()
+    _sync()
+    ref = gated_ref(x, wg.detach(), wu.detach(), "silu", dh)
+    for got in (grads, (wg.grad, wu.grad)):
+        check(got[0], ref[2])
+        check(got[1], ref[3])
+    assert live.requires_grad
+
+
+def test_make_graphed_callables():
+    """torch's own way to capture a module's forward and backward pass."""
+    from opengda_b200.ops.ffn import gated_linear
+
+    class Block(torch.nn.Module):
+        def __init__(self, wg, wu):
+            super().__init__()
+            self.wg, self.wu = torch.nn.Parameter(wg), torch.nn.Parameter(wu)
+
+        def forward(self, x):
+            return gated_linear(x, self.wg, self.wu, act="gelu")
+
+    x, wg, wu, dh = _make(70, 264, 130, torch.bfloat16, seed=5)
+    block = Block(wg, wu)
+    graphed = torch.cuda.make_graphed_callables(block, (x.clone().requires_grad_(True),))
+    for seed in (6, 7):
+        x, _, _, dh = _make(70, 264, 130, torch.bfloat16, seed=seed)
+        x.requires_grad_(True)
+        h = graphed(x)
+        got = (h.detach().clone(), *(t.clone() for t in torch.autograd.grad(h, (x, block.wg, block.wu), dh)))
+        _sync()
+        for t, r in zip(got, gated_ref(x.detach(), wg, wu, "gelu", dh)):
+            check(t, r)
